@@ -18,8 +18,7 @@ import random
 import torch
 
 own = False                    # False: elementary torch operations; True: the framework's kernels
-if own:
-    from hymt2sharp_b200.kernels import ops
+ops = None                     # the framework's operators, imported by the first pass that calls them
 
 DEV = "cuda:0"
 EPS = 1e-5
@@ -265,7 +264,10 @@ def _own(st):
 
 
 def run(state):
+    global ops
     if own:
+        if ops is None:
+            from hymt2sharp_b200.kernels import ops
         return _own(state)
     return _plain(state)
 
