@@ -37,7 +37,11 @@ _library = None
 _DECLARED = {"hymt2_gemm_tc_norm": "pippiiilllipl" "pippp" "iifppip" "iffp",
              "hymt2_gemm_tc_rope_kv": "ppiillpppp" "iipppppipp" "ifiiipppiif",
              "hymt2_attention_prefill_tc": "pppplpiipppiiiiiifipp",
-             "hymt2_gemm_f32_tc": "pppiiillliplpp" "iffp"}
+             "hymt2_gemm_f32_tc": "pppiiillliplpp" "iffp",
+             "hymt2_quantize_q8": "plppiliip",
+             "hymt2_dequantize_q8": "pilplpiip",
+             "hymt2_rmsnorm_q8": "plppilpilplpiiifp",
+             "hymt2_gemm_q8_tc": "pippppiiillli" "pp" "iffp"}
 
 
 def _lib():
@@ -2360,3 +2364,126 @@ def dense_block(x, pre, residual, w_qkv, w_o, w_gate_up, w_down, q_gain, k_gain,
         dtype_code(following.gain.dtype) if following is not None else F32, pre.ss.shape[1] if pre else 0, ss.shape[1],
         cnt.numel() if cnt is not None else 0, qk_eps, pre.eps if pre else 0.0, norm2.eps, scale)
     _check(_lib().hymt2_dense_block(ctypes.byref(block), _stream()), "dense_block", 5, timed=False)
+
+
+# -- 8-bit integers with a scale a row --------------------------------------------------------------------------------------------
+Q8_MAX_INNER = 131071     # entries of a row that a product takes: 128 * 128 of them stay below 2^31
+
+
+def q8_rows(rows: int, width: int, device) -> torch.Tensor:
+    """Room for [rows, width] 8-bit integers in the layout of the 8-bit kernels: every row starts on 16 bytes.  (What lies between two
+    rows belongs to neither.)"""
+    return torch.empty((rows, -(-width // 16) * 16), dtype=torch.int8, device=device)[:, :width]
+
+
+def _q8(t: torch.Tensor, scale: torch.Tensor, name: str) -> int:
+    """Checks a matrix of 8-bit rows and its scales; the rows' distance."""
+    if t.dtype != torch.int8 or t.dim() != 2:
+        raise KernelError(f"{name} must be an int8 matrix, got {t.dtype} {tuple(t.shape)}")
+    rows, width = t.shape
+    ld = t.stride(0) if rows > 1 else -(-width // 16) * 16
+    if (t.stride(1) != 1 and width > 1) or ld % 16 or ld < width or t.data_ptr() % 16:
+        raise KernelError(f"{name}: rows of 8-bit integers are contiguous and start on 16 bytes (see q8_rows), got strides {t.stride()}")
+    if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] != rows or (scale.stride(0) != 1 and rows > 1):
+        raise KernelError(f"{name}: {rows} rows need as many float32 scales side by side, got {scale.dtype} {tuple(scale.shape)}")
+    return ld
+
+
+def _plain_rows(t: torch.Tensor, name: str, shape) -> int:
+    """Checks a float32 or bfloat16 matrix with contiguous rows; the rows' distance."""
+    if t.dim() != 2 or t.shape != shape:
+        raise KernelError(f"{name} must be a {tuple(shape)} matrix, got {tuple(t.shape)}")
+    rows, width = t.shape
+    ld = t.stride(0) if rows > 1 else width
+    if (t.stride(1) != 1 and width > 1) or ld < width:
+        raise KernelError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
+    return ld
+
+
+def _on_current_device(what: str, *tensors) -> None:
+    here = tensors[0].get_device()
+    if here < 0 or any(t is not None and t.get_device() != here for t in tensors) or here != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: all operands lie on the current CUDA device, got {', '.join(str(t.device) for t in tensors if t is not None)}")
+
+
+def quantize_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor) -> None:
+    """Rows of x (float32 or bfloat16 [rows, width]) as 8-bit integers with a scale each:  q = 127 x / max|x| rounded to the nearest whole
+    number (ties to even, decided by the numbers as they are stored),  scale = max|x| / 127;  q * scale stands for x.  A row of zeros has the scale
+    0, a row that holds a NaN or an infinity the scale NaN and zeros.  A weight matrix's rows are its output channels."""
+    ldq = _q8(q, scale, "q")
+    ldx = _plain_rows(x, "x", q.shape)
+    rows, width = q.shape
+    code = dtype_code(x.dtype)
+    if width == 0:
+        raise KernelError("quantize_q8: rows without entries")
+    _on_current_device("quantize_q8", q, scale, x)
+    if rows == 0:
+        return
+    _check(_lib().hymt2_quantize_q8(q.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(), code, ldx, rows, width, _raw_stream()), "quantize_q8")
+
+
+def dequantize_q8(out: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """out (float32 or bfloat16) = q * scale: what rows of 8-bit integers stand for."""
+    ldq = _q8(q, scale, "q")
+    ldy = _plain_rows(out, "out", q.shape)
+    rows, width = q.shape
+    code = dtype_code(out.dtype)
+    _on_current_device("dequantize_q8", out, q, scale)
+    if rows == 0 or width == 0:
+        return
+    _check(_lib().hymt2_dequantize_q8(out.data_ptr(), code, ldy, q.data_ptr(), ldq, scale.data_ptr(), rows, width, _raw_stream()), "dequantize_q8")
+
+
+def rmsnorm_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, gain: torch.Tensor, eps: float, add: torch.Tensor | None = None,
+               total: torch.Tensor | None = None) -> None:
+    """t = x + add in x's type (t = x without `add`);  q, scale = the 8-bit rows of rmsnorm(t) * gain (quantize_q8).  `total` receives t; it may be x
+    itself: the residual's rows then take the addition in place.  The root mean square goes into the scale, so the integers are those of t * gain."""
+    ldq = _q8(q, scale, "q")
+    ldx = _plain_rows(x, "x", q.shape)
+    rows, width = q.shape
+    if gain.dim() != 1 or gain.shape[0] != width or (width > 1 and gain.stride(0) != 1):
+        raise KernelError(f"rmsnorm_q8: the gain must hold {width} entries side by side, got {tuple(gain.shape)}")
+    ldadd = ldt = 0
+    if add is not None:
+        ldadd = _plain_rows(add, "add", q.shape)
+    if total is not None:
+        ldt = _plain_rows(total, "total", q.shape)
+        if add is None or total.dtype != x.dtype:
+            raise KernelError("rmsnorm_q8: `total` takes the sum of x and `add` in x's type")
+    x_code, add_code, gain_code = dtype_code(x.dtype), dtype_code(add.dtype) if add is not None else F32, dtype_code(gain.dtype)
+    if width == 0:
+        raise KernelError("rmsnorm_q8: rows without entries")
+    _on_current_device("rmsnorm_q8", q, scale, x, gain, add, total)
+    if rows == 0:
+        return
+    _check(_lib().hymt2_rmsnorm_q8(q.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(), x_code, ldx, _address(add), add_code, ldadd, _address(total), ldt,
+                                   gain.data_ptr(), gain_code, rows, width, eps, _raw_stream()), "rmsnorm_q8")
+
+
+def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int, status: torch.Tensor,
+               glu: GluRule | None = None, glu_bias: torch.Tensor | None = None) -> None:
+    """out[t, n] = epilogue(a_scale[t] * w_scale[n] * sum_k a[t, k] * w[n, k]): 8-bit rows of tokens with 8-bit rows of weights, the sums exact
+    in 32-bit integers, the rest in float32.  Store (float32 or bfloat16), accumulate (float32) or SwiGLU (w and w_scale have 2N rows, gates first;
+    `glu` and `glu_bias` as for gemm_tc, with outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row."""
+    lda, ldw = _q8(a, a_scale, "a"), _q8(w, w_scale, "w")
+    T, K = a.shape
+    gated = epilogue == EPILOGUE_SWIGLU
+    N = w.shape[0] // 2 if gated else w.shape[0]
+    ldo = _plain_rows(out, "out", (T, N))
+    if w.shape[1] != K or (gated and w.shape[0] % 2) or not 0 < K <= Q8_MAX_INNER:
+        raise KernelError(f"gemm_q8_tc: a {tuple(a.shape)} and w {tuple(w.shape)} do not go together (rows of equal length, 1 to {Q8_MAX_INNER} entries, "
+                          f"gate and up rows of equal number)")
+    if epilogue not in (EPILOGUE_STORE, EPILOGUE_ACCUMULATE, EPILOGUE_SWIGLU) or (epilogue == EPILOGUE_ACCUMULATE and out.dtype != torch.float32):
+        raise KernelError(f"gemm_q8_tc: epilogue {epilogue} into {out.dtype} is not built (sums are added into float32)")
+    if status.dtype != torch.int32:
+        raise KernelError("gemm_q8_tc: the status word is an int32 tensor")
+    code = dtype_code(out.dtype)
+    _on_current_device("gemm_q8_tc", out, a, a_scale, w, w_scale, status, glu_bias)
+    rule = (0, 0.0, 1.0, 0)
+    if glu is not None or glu_bias is not None:
+        args = _glu_arguments(glu, glu_bias, N, epilogue)
+        rule = (args[0].value, args[1].value, args[2].value, _address(glu_bias))
+    if T == 0 or N == 0:
+        return
+    _check(_lib().hymt2_gemm_q8_tc(out.data_ptr(), code, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), T, N, K, lda, ldw, ldo,
+                                   epilogue, status.data_ptr(), _raw_stream(), *rule), "gemm_q8_tc")
