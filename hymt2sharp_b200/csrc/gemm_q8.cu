@@ -1,20 +1,34 @@
-// Products of 8-bit integers with a scale for each token and one for each output channel:
+// Products of 8-bit integers with a scale for each token and one for each output channel, on the tensor cores of sm_100a:
 //   C[t, n] = epilogue(a_scale[t] w_scale[n] sum_k A[t, k] W[n, k])
-// The sums are 32-bit integers and exact (K up to 131,071: 128 * 128 * K stays below 2^31), so a row's result does not depend on how K is cut,
-// nor on the other rows.  Epilogues: store (float32 or bfloat16), add into float32 C, gated (W holds N gate rows, then N up rows).
-#include "common.cuh"
+// The sums are 32-bit integers in tensor memory (`tcgen05.mma.kind::i8`, 32 entries of K an instruction) and exact (K up to 131,071: 128 * 128 * K stays
+// below 2^31), so a row's result does not depend on how K is cut, nor on the other rows.  The scaling is (sum * a_scale) * w_scale in float32.
+// Epilogues: store (float32 or bfloat16), add into float32 C, gated (W holds N gate rows, then N up rows; see GluRule).
+//
+// Operand tiles of 128 entries of K (128 bytes a row, 128-byte swizzle) come into shared memory by TMA through a ring of stages guarded by mbarriers; one
+// thread issues the copies, one the MMAs, the other warps drain the accumulators.  Two kernels:
+//   few tokens    the 128-row side holds weight rows, the other 16 to 128 tokens; K is cut over a cluster of up to 8 CTAs, whose partial sums meet
+//                 through distributed shared memory (gemm_q8_few_kernel).  Bound by the weights' way from memory.
+//   many tokens   persistent pairs of CTAs (cta_group::2) on tiles of 256 tokens (gemm_q8_pair_kernel).  Bound by the tensor cores.
+// Rows, tokens and K beyond the matrices are zeros by TMA and masked in the epilogue.  Every wait on an mbarrier is bounded (see tc_common.cuh).
+#include "tc_common.cuh"
 
 namespace {
 
 enum { EPI_STORE = 0, EPI_ACCUMULATE = 1, EPI_GATED = 2 };
-constexpr int MAX_K = 131071, TILE = 64, TILE_K = 64;
+constexpr int MAX_K = 131071, BLOCK_K = 128, UMMA_K = 32, TILE_M = 128, MAX_STAGES = 8;
+constexpr int A_TILE_BYTES = TILE_M * BLOCK_K;
+// instruction descriptor: D 32-bit integers, A and B signed 8-bit integers, both K-major
+__host__ __device__ constexpr uint32_t idesc_q8(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
 struct GemmQ8Params {
     void* C;
-    const int8_t *A, *W;
     const float *a_scale, *w_scale;
-    long lda, ldw, ldc;
+    long ldc;
     int T, N, K;
+    int bn, stages, splits, k_blocks_per_split;
+    int early;               // the weights were complete before the kernel in front was launched
+    int tma_out;             // many tokens: C leaves by TMA
+    int* status;
     GluRule glu;
 };
 
@@ -30,75 +44,594 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // glu_at of common.cuh, but a NaN stays one under the clamps: it says that the row held one before it became integers
 __device__ __forceinline__ float gated_at(const GluRule& r, float g, float u, int n, int N) {
-    if (r.bias) { g += r.bias[n]; u += r.bias[N + n]; }
+    if (r.bias) { g = __fadd_rn(g, r.bias[n]); u = __fadd_rn(u, r.bias[N + n]); }
     if (r.kind == GLU_SILU) return silu_mul(g, u);
     g = min_nan(g, r.limit);
     u = min_nan(max_nan(u, -r.limit), r.limit);
     return g / (1.0f + expf(-r.alpha * g)) * (u + 1.0f);
 }
+// (products of their own and no FMA with what follows: both kernels give the same bits)
+__device__ __forceinline__ float scaled(int sum, float a, float w) { return __fmul_rn(__fmul_rn((float)sum, a), w); }
+
+__device__ __forceinline__ void umma_q8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_q8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_pair_commit(uint32_t bar) {      // the barrier at this place in both CTAs
+    asm volatile(
+        "{\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t even_bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"((uint64_t)map), "r"(even_bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_even(uint32_t even_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_bar) : "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t local_addr, uint32_t rank) {
+    const float4 v = ld_cluster_f32x4(local_addr, rank);
+    return make_int4(__float_as_int(v.x), __float_as_int(v.y), __float_as_int(v.z), __float_as_int(v.w));
+}
+
+// --------------------------------------------------------------------------------------------
+// Few tokens: a CTA computes 128 weight rows (gated: 128 gate and 128 up rows) x BN tokens over its cut of K.
+// --------------------------------------------------------------------------------------------
+constexpr int FEW_THREADS = 192;       // warp 0 TMA, warp 1 MMAs, warps 2 to 5 the sums
+constexpr int MAX_RANKS = 8;           // a portable cluster
+
+template <int BN, int EPI, typename TC>
+__global__ void __launch_bounds__(FEW_THREADS)
+gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, GemmQ8Params p) {
+    constexpr int NUM_ACC = EPI == EPI_GATED ? 2 : 1;
+    constexpr int STAGE_BYTES = NUM_ACC * A_TILE_BYTES + BN * BLOCK_K;
+    constexpr int ACC_COLS = NUM_ACC * BN;
+    constexpr int TMEM_COLS = ACC_COLS <= 32 ? 32 : ACC_COLS;        // 32, 64, 128 or 256
+    constexpr uint32_t IDESC = idesc_q8(TILE_M, BN);
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 1];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+    const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stages = p.stages;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[MAX_STAGES]), done_bar = smem_u32(&bars[2 * MAX_STAGES]);
+    volatile int* abort_flag = &abort_s;
+    const int num_k_blocks = (p.K + BLOCK_K - 1) / BLOCK_K;
+    const int kb_begin = blockIdx.z * p.k_blocks_per_split;
+    const int my_blocks = max(0, min(num_k_blocks, kb_begin + p.k_blocks_per_split) - kb_begin);
+    const int n0 = blockIdx.x * TILE_M, t0 = blockIdx.y * BN;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(done_bar, 1);
+        abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_base_s;
+    pdl_launch_dependents();            // (behind the allocation: a CTA of the next kernel cannot have taken this one's tensor memory)
+
+    if (warp == 0 && elect_one()) {
+        auto load_weights = [&](int i) {
+            const uint32_t bar = full0 + 8 * (i % stages), dst = tiles + (i % stages) * STAGE_BYTES;
+            const int k = (kb_begin + i) * BLOCK_K;
+            tma_load_2d(dst, &map_w, bar, k, n0);
+            if (NUM_ACC == 2) tma_load_2d(dst + A_TILE_BYTES, &map_w, bar, k, p.N + n0);
+        };
+        auto load_tokens = [&](int i) {
+            tma_load_2d(tiles + (i % stages) * STAGE_BYTES + NUM_ACC * A_TILE_BYTES, &map_a, full0 + 8 * (i % stages), (kb_begin + i) * BLOCK_K, t0);
+        };
+        // the first ring of weights before the wait for the kernel in front, where they do not come from it
+        const int ahead = min(stages, my_blocks);
+        if (!p.early) pdl_wait();
+        for (int i = 0; i < ahead; i++) {
+            mbar_expect_tx(full0 + 8 * i, STAGE_BYTES);
+            load_weights(i);
+        }
+        if (p.early) pdl_wait();
+        for (int i = 0; i < ahead; i++) load_tokens(i);
+        int issued = ahead;
+        for (int i = ahead; i < my_blocks; i++) {
+            const int s = i % stages;
+            if (!mbar_wait(empty0 + 8 * s, ((i / stages) & 1) ^ 1, abort_flag, p.status, 151)) break;
+            mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
+            load_weights(i);
+            load_tokens(i);
+            issued = i + 1;
+        }
+        if (*abort_flag)        // copies that are in flight must land before the CTA's shared memory goes away
+            for (int i = max(0, issued - stages); i < issued; i++)
+                for (uint32_t t = 0; t < (1u << 16) && !mbar_try_wait(full0 + 8 * (i % stages), (i / stages) & 1); t++) {}
+    } else if (warp == 1 && elect_one()) {
+        constexpr uint64_t K_STEP = UMMA_K >> 4, A2_STEP = A_TILE_BYTES >> 4, B_STEP = (NUM_ACC * A_TILE_BYTES) >> 4;
+        const uint64_t desc0 = desc_k_major(tiles);
+        uint32_t s = 0, phase = 0;
+        for (int i = 0; i < my_blocks; i++) {
+            if (!mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t adesc = desc0 + (uint64_t)s * (uint64_t)(STAGE_BYTES >> 4), bdesc = adesc + B_STEP;
+#pragma unroll
+            for (int k = 0; k < BLOCK_K / UMMA_K; k++) {
+                umma_q8(tmem_base, adesc + k * K_STEP, bdesc + k * K_STEP, IDESC, i > 0 || k > 0);
+                if (NUM_ACC == 2) umma_q8(tmem_base + BN, adesc + A2_STEP + k * K_STEP, bdesc + k * K_STEP, IDESC, i > 0 || k > 0);
+            }
+            umma_commit(empty0 + 8 * s);
+            if (++s == (uint32_t)stages) { s = 0; phase ^= 1; }
+        }
+        umma_commit(done_bar);
+    } else if (warp >= 2) {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        pdl_wait();             // C may still be in use by the kernel in front, and the scales come from it
+        TC* C = (TC*)p.C;
+        const int cols = min(BN, p.T - t0);
+        // a lane of the fold has four neighbouring weight rows
+        const int n4 = n0 + 4 * lane;
+        float sw[NUM_ACC][4];
+#pragma unroll
+        for (int h = 0; h < NUM_ACC; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sw[h][i] = n4 + i < p.N ? p.w_scale[(size_t)h * p.N + n4 + i] : 0.f;
+        const bool vec = n4 + 4 <= p.N && (p.ldc & 3) == 0 && ((uintptr_t)C & (4 * sizeof(TC) - 1)) == 0;
+
+        const bool ok = my_blocks > 0 ? mbar_wait(done_bar, 0, abort_flag, p.status, 153) : true;
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // the sums -> this CTA's shared memory (the ring is free now), [column][row]
+        constexpr int CH = BN >= 32 ? 32 : 16;
+#pragma unroll 1
+        for (int h = 0; h < NUM_ACC; h++)
+#pragma unroll 1
+            for (int c = 0; c < cols; c += CH) {
+                float g[CH];
+                if (ok && my_blocks > 0) {
+                    if constexpr (CH == 32) tmem_load32(lane_addr + h * BN + c, g);
+                    else tmem_load16(lane_addr + h * BN + c, g);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < CH; j++) g[j] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < CH; j++)
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((h * BN + c + j) * TILE_M + row) * 4), "f"(g[j]) : "memory");
+            }
+        __syncwarp();
+        if (p.splits > 1) cluster_sync_all();
+        else asm volatile("bar.sync 1, 128;" ::: "memory");
+        // every CTA of the cluster takes a share of the tokens, adds all ranks' sums for them and writes them out; a warp has a token,
+        // a lane four weight rows
+        const int share = (cols + p.splits - 1) / p.splits;
+        const int c_begin = (int)blockIdx.z * share, c_end = min(cols, c_begin + share);
+#pragma unroll 1
+        for (int c = c_begin + quarter; c < c_end; c += 4) {
+            int4 part[NUM_ACC][MAX_RANKS];
+#pragma unroll
+            for (int r = 0; r < MAX_RANKS; r++)
+#pragma unroll
+                for (int h = 0; h < NUM_ACC; h++)
+                    part[h][r] = r < p.splits ? ld_cluster_s32x4(tiles + ((h * BN + c) * TILE_M + 4 * lane) * 4, r) : make_int4(0, 0, 0, 0);
+            const float sa = p.a_scale[t0 + c];
+            float y[NUM_ACC][4];
+#pragma unroll
+            for (int h = 0; h < NUM_ACC; h++) {
+                int4 sum = part[h][0];
+#pragma unroll
+                for (int r = 1; r < MAX_RANKS; r++) { sum.x += part[h][r].x; sum.y += part[h][r].y; sum.z += part[h][r].z; sum.w += part[h][r].w; }
+                y[h][0] = scaled(sum.x, sa, sw[h][0]); y[h][1] = scaled(sum.y, sa, sw[h][1]);
+                y[h][2] = scaled(sum.z, sa, sw[h][2]); y[h][3] = scaled(sum.w, sa, sw[h][3]);
+            }
+            TC* dst = C + (size_t)(t0 + c) * p.ldc + n4;
+            if constexpr (EPI == EPI_GATED) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (n4 + i < p.N) y[0][i] = gated_at(p.glu, y[0][i], y[1][i], n4 + i, p.N);
+            }
+            if (vec) {
+                if constexpr (EPI == EPI_ACCUMULATE) {
+                    const float4 old = *reinterpret_cast<const float4*>(dst);
+                    y[0][0] = __fadd_rn(old.x, y[0][0]); y[0][1] = __fadd_rn(old.y, y[0][1]);
+                    y[0][2] = __fadd_rn(old.z, y[0][2]); y[0][3] = __fadd_rn(old.w, y[0][3]);
+                }
+                if constexpr (sizeof(TC) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0][0], y[0][1], y[0][2], y[0][3]);
+                else {
+                    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(y[0][0], y[0][1]), __floats2bfloat162_rn(y[0][2], y[0][3])};
+                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (n4 + i < p.N) dst[i] = from_float<TC>(EPI == EPI_ACCUMULATE ? __fadd_rn(to_float(dst[i]), y[0][i]) : y[0][i]);
+            }
+        }
+        __syncwarp();
+    }
+    if (p.splits > 1) {         // no CTA leaves before its peers have read its sums; the other warps come to both barriers too
+        __syncwarp();
+        if (warp < 2) cluster_sync_all();
+        cluster_sync_all();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// --------------------------------------------------------------------------------------------
+// Many tokens: persistent pairs of CTAs walk tiles of 256 tokens x bn weight rows (gated: bn / 2 gate and bn / 2 up rows), token tiles fastest.  A CTA holds
+// its 128 tokens and half of the weight rows; the even CTA issues the MMAs of both.  Two accumulators in tensor memory alternate.
+// --------------------------------------------------------------------------------------------
+constexpr int PAIR_THREADS = 320;      // warp 0 TMA, warp 1 MMAs, warps 2 to 9 the sums: each has 32 tokens and every other piece of columns
+constexpr int PAIR_BN = 256;           // the widest tile: the accumulators lie so many columns apart
+constexpr int PIECE_BYTES = 64;        // a token's piece of output columns: 32 of bfloat16, 16 of float32
+constexpr int OUT_BUFFER = 32 * PIECE_BYTES, OUT_BYTES = 8 * 2 * OUT_BUFFER;   // a warp has two buffers that TMA writes out
 
 template <int EPI, typename TC>
-__global__ void gemm_q8_kernel(GemmQ8Params p) {
-    __shared__ int a_s[TILE][TILE_K / 4 + 1], w_s[2][TILE][TILE_K / 4 + 1];
-    constexpr int PARTS = EPI == EPI_GATED ? 2 : 1;
-    pdl_wait();
-    pdl_launch_dependents();
-    const int t0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    int acc[PARTS][4][4] = {};
-    auto word = [&](const int8_t* m, long ld, long row, bool in, int k) {
-        int v = 0;
-        if (in && k < p.K) {
-            v = *reinterpret_cast<const int*>(m + row * ld + k);          // (rows lie on 16 bytes, so the word is the matrix's own memory)
-            if (k + 4 > p.K) v &= (1 << (8 * (p.K - k))) - 1;
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
+                    GemmQ8Params p) {
+    constexpr bool GATED = EPI == EPI_GATED;
+    constexpr int PIECE = PIECE_BYTES / (int)sizeof(TC);
+    const int bn = p.bn, B_TILE_BYTES = bn / 2 * BLOCK_K, STAGE_BYTES = A_TILE_BYTES + B_TILE_BYTES;
+    const int OUT_COLS = GATED ? bn / 2 : bn;
+    const uint32_t IDESC = idesc_q8(2 * TILE_M, bn);
+    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2, rank = blockIdx.x % 2;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 4];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+    const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stages = p.stages;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[MAX_STAGES]);
+    const uint32_t acc_full0 = smem_u32(&bars[2 * MAX_STAGES]), acc_empty0 = acc_full0 + 16;
+    volatile int* abort_flag = &abort_s;
+    const int num_k_blocks = (p.K + BLOCK_K - 1) / BLOCK_K;
+    const int tiles_t = (p.T + 2 * TILE_M - 1) / (2 * TILE_M), tiles_n = (p.N + OUT_COLS - 1) / OUT_COLS, num_tiles = tiles_t * tiles_n;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
         }
-        return v;
-    };
-    for (int k0 = 0; k0 < p.K; k0 += TILE_K) {
-        for (int i = threadIdx.x; i < TILE * TILE_K / 4; i += 256) {
-            const int row = i / (TILE_K / 4), k = i % (TILE_K / 4);
-            a_s[row][k] = word(p.A, p.lda, t0 + row, t0 + row < p.T, k0 + 4 * k);
-            for (int h = 0; h < PARTS; h++) w_s[h][row][k] = word(p.W, p.ldw, (long)h * p.N + n0 + row, n0 + row < p.N, k0 + 4 * k);
+        for (int b = 0; b < 2; b++) {
+            mbar_init(acc_full0 + 8 * b, 1);
+            mbar_init(acc_empty0 + 8 * b, 16);      // the warps of both CTAs
         }
-        __syncthreads();
-        for (int k = 0; k < TILE_K / 4; k++)
-            for (int i = 0; i < 4; i++)
-                for (int h = 0; h < PARTS; h++)
-                    for (int j = 0; j < 4; j++) acc[h][i][j] = __dp4a(a_s[ty * 4 + i][k], w_s[h][tx * 4 + j][k], acc[h][i][j]);
-        __syncthreads();
+        abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    TC* C = (TC*)p.C;
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int t = t0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (t >= p.T || n >= p.N) continue;
-            const float y = (float)acc[0][i][j] * p.a_scale[t] * p.w_scale[n];
-            TC* dst = C + (size_t)t * p.ldc + n;
-            if (EPI == EPI_STORE) *dst = from_float<TC>(y);
-            else if (EPI == EPI_ACCUMULATE) *dst = from_float<TC>(to_float(*dst) + y);
-            else *dst = from_float<TC>(gated_at(p.glu, y, (float)acc[PARTS - 1][i][j] * p.a_scale[t] * p.w_scale[p.N + n], n, p.N));
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(2 * PAIR_BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync_all();                 // both CTAs' barriers and tensor memory are there
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_base_s;
+    pdl_launch_dependents();            // (behind the allocation: a CTA of the next kernel cannot have taken this one's tensor memory)
+
+    if (warp == 0 && elect_one()) {
+        uint32_t s = 0, round = 0;
+        const uint32_t even_full0 = at_rank(full0, 0);
+        bool first = true;
+        if (!p.early) pdl_wait();
+        for (int tile = pair; tile < num_tiles && !*abort_flag; tile += pairs) {
+            const int a_row = (tile % tiles_t) * 2 * TILE_M + rank * TILE_M;
+            // the even CTA brings the first half of the weight rows, the odd one the second; of gated rows the gates and the ups
+            const int w_row = (tile / tiles_t) * OUT_COLS + rank * (GATED ? p.N : bn / 2);
+            for (int kb = 0; kb < num_k_blocks; kb++) {
+                if (round > 0 && !mbar_wait(empty0 + 8 * s, (round & 1) ^ 1, abort_flag, p.status, 151)) break;
+                const uint32_t bar = even_full0 + 8 * s, a_dst = tiles + s * STAGE_BYTES;
+                if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
+                tma_load_2d_pair(a_dst + A_TILE_BYTES, &map_w, bar, kb * BLOCK_K, w_row);
+                if (first && p.early) pdl_wait();
+                first = false;
+                tma_load_2d_pair(a_dst, &map_a, bar, kb * BLOCK_K, a_row);
+                if (++s == (uint32_t)stages) { s = 0; round++; }
+            }
         }
+        if (rank == 0 && *abort_flag)   // copies in flight (both CTAs' are counted here) must land before the shared memory goes away
+            for (int back = 0; back < stages && (round > 0 || s > 0); back++) {
+                if (s == 0) { s = stages; round--; }
+                s--;
+                for (uint32_t t = 0; t < (1u << 16) && !mbar_try_wait(full0 + 8 * s, round & 1); t++) {}
+            }
+    } else if (warp == 1 && rank == 0 && elect_one()) {
+        const uint64_t desc0 = desc_k_major(tiles);
+        uint32_t s = 0, phase = 0;
+        int j = 0;
+        for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
+            const int buf = j & 1;
+            if (j >= 2 && !mbar_wait(acc_empty0 + 8 * buf, (uint32_t)(((j >> 1) - 1) & 1), abort_flag, p.status, 154)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            bool ok = true;
+            for (int kb = 0; kb < num_k_blocks; kb++) {
+                if (!(ok = mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t adesc = desc0 + (uint64_t)s * (uint64_t)(STAGE_BYTES >> 4), bdesc = adesc + (A_TILE_BYTES >> 4);
+#pragma unroll
+                for (int k = 0; k < BLOCK_K / UMMA_K; k++)
+                    umma_q8_pair(tmem_base + buf * PAIR_BN, adesc + k * (UMMA_K >> 4), bdesc + k * (UMMA_K >> 4), IDESC, kb > 0 || k > 0);
+                umma_pair_commit(empty0 + 8 * s);
+                if (++s == (uint32_t)stages) { s = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            umma_pair_commit(acc_full0 + 8 * buf);
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3, side = (warp - 2) >> 2;
+        const uint32_t stage_out = tiles + stages * STAGE_BYTES + (warp - 2) * 2 * OUT_BUFFER;
+        pdl_wait();             // C may still be in use by the kernel in front, and the scales come from it
+        TC* C = (TC*)p.C;
+        int j = 0, used = 0;
+        for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
+            const int buf = j & 1;
+            const int t_first = (tile % tiles_t) * 2 * TILE_M + rank * TILE_M + quarter * 32, t = t_first + lane;
+            const int n_first = (tile / tiles_t) * OUT_COLS;
+            const float sa = t < p.T ? p.a_scale[t] : 0.f;
+            const bool landed = mbar_wait(acc_full0 + 8 * buf, (uint32_t)((j >> 1) & 1), abort_flag, p.status, 153);
+            if (!__all_sync(0xffffffffu, landed)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * PAIR_BN;
+#pragma unroll 1
+            for (int c = side * PIECE; c < OUT_COLS; c += 2 * PIECE) {
+                const int n = n_first + c;
+                if (n >= p.N || t_first >= p.T) break;               // (the same for the whole warp)
+                float y[PIECE], u[GATED ? PIECE : 1];
+                if constexpr (PIECE == 32) {
+                    tmem_load32(lane_addr + c, y);
+                    if constexpr (GATED) tmem_load32(lane_addr + bn / 2 + c, u);
+                } else {
+                    tmem_load16(lane_addr + c, y);
+                    if constexpr (GATED) tmem_load16(lane_addr + bn / 2 + c, u);
+                }
+                auto scale_all = [&](float* v, const float* w) {
+                    if (n + PIECE <= p.N && (uintptr_t)w % 16 == 0) {
+#pragma unroll
+                        for (int q = 0; q < PIECE; q += 4) {
+                            const float4 s4 = __ldg(reinterpret_cast<const float4*>(w + q));
+                            v[q] = scaled(__float_as_int(v[q]), sa, s4.x); v[q + 1] = scaled(__float_as_int(v[q + 1]), sa, s4.y);
+                            v[q + 2] = scaled(__float_as_int(v[q + 2]), sa, s4.z); v[q + 3] = scaled(__float_as_int(v[q + 3]), sa, s4.w);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < PIECE; q++) v[q] = scaled(__float_as_int(v[q]), sa, n + q < p.N ? __ldg(w + q) : 0.f);
+                    }
+                };
+                scale_all(y, p.w_scale + n);
+                if constexpr (GATED) {
+                    scale_all(u, p.w_scale + (size_t)p.N + n);
+#pragma unroll
+                    for (int q = 0; q < PIECE; q++) y[q] = n + q < p.N ? gated_at(p.glu, y[q], u[q], n + q, p.N) : 0.f;
+                }
+                if (p.tma_out) {
+                    // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them; the buffer of two pieces ago has been read
+                    const uint32_t out = stage_out + (used & 1) * OUT_BUFFER;
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const uint32_t at = out + lane * PIECE_BYTES + ((q ^ ((lane >> 1) & 3)) << 4);
+                        uint32_t w[4];
+                        if constexpr (sizeof(TC) == 4) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) w[i] = __float_as_uint(y[4 * q + i]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(y[8 * q + 2 * i], y[8 * q + 2 * i + 1]);
+                                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (EPI == EPI_ACCUMULATE)
+                            asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"((uint64_t)&map_c), "r"(n), "r"(t_first), "r"(out) : "memory");
+                        else
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"((uint64_t)&map_c), "r"(n), "r"(t_first), "r"(out) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                    used++;
+                } else if (t < p.T) {
+                    TC* dst = C + (size_t)t * p.ldc + n;
+#pragma unroll
+                    for (int q = 0; q < PIECE; q++)
+                        if (n + q < p.N) dst[q] = from_float<TC>(EPI == EPI_ACCUMULATE ? __fadd_rn(to_float(dst[q]), y[q]) : y[q]);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_even(at_rank(acc_empty0 + 8 * buf, 0));
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");      // what left by TMA is in memory
+        __syncwarp();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    __syncwarp();
+    cluster_sync_all();                 // neither CTA leaves while the other may still arrive at its barriers
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * PAIR_BN) : "memory");
+    }
+}
+
+// --------------------------------------------------------------------------------------------
+// host side
+// --------------------------------------------------------------------------------------------
+// [rows, cols] 8-bit integers, rows ld bytes apart: boxes of 128 columns x box_rows rows, 128-byte swizzle, zeros outside the matrix
+bool make_map_q8(CUtensorMap* map, const void* base, long rows, long cols, long ld, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {BLOCK_K, (cuuint32_t)box_rows}, elem[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// the output [rows, cols]: boxes of 64 bytes x 32 rows, 64-byte swizzle
+bool make_map_out(CUtensorMap* map, void* base, bool bf16, long rows, long cols, long ld) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const int size = bf16 ? 2 : 4;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * size};
+    cuuint32_t box[2] = {(cuuint32_t)(PIECE_BYTES / size), 32}, elem[2] = {1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, base, dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan {
+    bool few;
+    int bn, stages, splits, k_blocks_per_split;
+    int tiles_n, tiles_t, ctas;
+    size_t smem;
+};
+
+Plan make_plan(int T, int N, int K, bool gated, int sm_count) {
+    Plan pl{};
+    const int k_blocks = (K + BLOCK_K - 1) / BLOCK_K;
+    pl.few = T <= 128;
+    pl.splits = 1;
+    pl.k_blocks_per_split = k_blocks;
+    if (pl.few) {
+        pl.bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+        pl.tiles_n = (N + TILE_M - 1) / TILE_M;
+        pl.tiles_t = (T + pl.bn - 1) / pl.bn;
+        const int tiles = pl.tiles_n * pl.tiles_t;
+        int want = 2 * sm_count / tiles;
+        want = want < 1 ? 1 : want > MAX_RANKS ? MAX_RANKS : want;
+        while (want > 1 && k_blocks / want < 2) want--;
+        pl.k_blocks_per_split = (k_blocks + want - 1) / want;
+        pl.splits = (k_blocks + pl.k_blocks_per_split - 1) / pl.k_blocks_per_split;
+        pl.ctas = tiles * pl.splits;
+        const int stage = (gated ? 2 : 1) * A_TILE_BYTES + pl.bn * BLOCK_K, sums = (gated ? 2 : 1) * pl.bn * TILE_M * 4;
+        int stages = 110 * 1024 / stage;
+        stages = stages > MAX_STAGES ? MAX_STAGES : stages;
+        stages = stages > pl.k_blocks_per_split ? pl.k_blocks_per_split : stages;
+        pl.stages = stages < 2 ? 2 : stages;
+        const size_t ring = (size_t)pl.stages * stage;
+        pl.smem = (ring > (size_t)sums ? ring : (size_t)sums) + 1024;
+        return pl;
+    }
+    pl.bn = PAIR_BN;
+    const int out = gated ? pl.bn / 2 : pl.bn;
+    pl.tiles_n = (N + out - 1) / out;
+    pl.tiles_t = (T + 2 * TILE_M - 1) / (2 * TILE_M);
+    const long tiles = (long)pl.tiles_n * pl.tiles_t;
+    const int pairs = sm_count / 2;
+    pl.ctas = 2 * (int)(tiles < pairs ? tiles : pairs);
+    const int stage = A_TILE_BYTES + pl.bn / 2 * BLOCK_K;
+    const int stages = (225 * 1024 - OUT_BYTES) / stage;
+    pl.stages = stages > MAX_STAGES ? MAX_STAGES : stages;
+    pl.smem = (size_t)pl.stages * stage + OUT_BYTES + 1024;
+    return pl;
+}
+
+int sm_count_of_current_device() {
+    static int cached[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 148;
+    if (!cached[dev]) cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev);
+    return cached[dev] > 0 ? cached[dev] : 148;
+}
+
+template <auto KERNEL, typename... Args>
+int launch_cluster(dim3 grid, int threads, dim3 cluster, size_t smem, cudaStream_t stream, Args... args) {
+    static bool configured[64] = {};       // per kernel and device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaError_t e = cudaSuccess;
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = hymt2_pdl_enabled() ? 1 : 0;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster.x;
+        attr[1].val.clusterDim.y = cluster.y;
+        attr[1].val.clusterDim.z = cluster.z;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
+    }
+    if (e != cudaSuccess) { hymt2_set_error("gemm_q8_tc: %s", cudaGetErrorString(e)); return HYMT2_ERR_LAUNCH; }
+    return hymt2_check_launch("gemm_q8_tc");
+}
+
+template <int EPI, typename TC>
+int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const Plan& pl, cudaStream_t stream) {
+    CUtensorMap ma, mw, mc{};
+    const long w_rows = EPI == EPI_GATED ? 2L * p.N : p.N;
+    HYMT2_REQUIRE(make_map_q8(&ma, A, p.T, p.K, lda, pl.few ? pl.bn : TILE_M) && make_map_q8(&mw, W, w_rows, p.K, ldw, pl.few ? TILE_M : pl.bn / 2),
+                  "gemm_q8_tc: cuTensorMapEncodeTiled refused the operands");
+    if (pl.few) {
+        const dim3 grid(pl.tiles_n, pl.tiles_t, pl.splits), cluster(1, 1, pl.splits);
+        switch (pl.bn) {
+            case 16: return launch_cluster<gemm_q8_few_kernel<16, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
+            case 32: return launch_cluster<gemm_q8_few_kernel<32, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
+            case 64: return launch_cluster<gemm_q8_few_kernel<64, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
+            default: return launch_cluster<gemm_q8_few_kernel<128, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
+        }
+    }
+    // (TMA writes whole pieces of 16 bytes: where the last of a row is not whole, it would write what lies between the rows)
+    p.tma_out = (uintptr_t)p.C % 16 == 0 && p.ldc * (long)sizeof(TC) % 16 == 0 && p.N * (long)sizeof(TC) % 16 == 0;
+    if (p.tma_out) HYMT2_REQUIRE(make_map_out(&mc, p.C, sizeof(TC) == 2, p.T, p.N, p.ldc), "gemm_q8_tc: cuTensorMapEncodeTiled refused the output");
+    return launch_cluster<gemm_q8_pair_kernel<EPI, TC>>(dim3(pl.ctas), PAIR_THREADS, dim3(2, 1, 1), pl.smem, stream, ma, mw, mc, p);
 }
 
 }  // namespace
 
-// C[T, N] (ldc) = epilogue(A[T, K] (lda) · W[N, K]^T (ldw)) with the scales of A's rows and W's; gated: W has 2N rows.
+// C[T, N] (ldc) = epilogue(A[T, K] (lda) · W[N, K]^T (ldw)) with the scales of A's rows and W's; gated: W has 2N rows.  weights_settled: W and its
+// scales were complete before the kernel in front of this one was launched, so they are fetched while that one still runs.
 HYMT2_API int hymt2_gemm_q8_tc(void* C, int c_dtype, const void* A, const float* a_scale, const void* W, const float* w_scale, int T, int N, int K,
-                               long lda, long ldw, long ldc, int epilogue, int* status, cudaStream_t stream, int glu_kind, float glu_limit,
-                               float glu_alpha, const float* glu_bias) {
+                               long lda, long ldw, long ldc, int epilogue, int weights_settled, int* status, cudaStream_t stream, int glu_kind,
+                               float glu_limit, float glu_alpha, const float* glu_bias) {
     if (T == 0 || N == 0) return HYMT2_OK;
     HYMT2_REQUIRE(T > 0 && N > 0 && K > 0 && K <= MAX_K, "gemm_q8_tc: bad sizes T=%d N=%d K=%d (K is at most %d)", T, N, K, MAX_K);
     HYMT2_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && (uintptr_t)A % 16 == 0 && (uintptr_t)W % 16 == 0, "gemm_q8_tc: rows must start on 16 bytes");
-    const GemmQ8Params p{C, (const int8_t*)A, (const int8_t*)W, a_scale, w_scale, lda, ldw, ldc, T, N, K, GluRule{glu_kind, glu_limit, glu_alpha, glu_bias}};
-    const dim3 grid((T + TILE - 1) / TILE, (N + TILE - 1) / TILE);
-    if (epilogue == EPI_ACCUMULATE) {
-        HYMT2_REQUIRE(c_dtype == HYMT2_F32, "gemm_q8_tc: sums are added into float32 only");
-        launch_pdl(gemm_q8_kernel<EPI_ACCUMULATE, float>, grid, dim3(256), 0, stream, p);
-    } else if (epilogue == EPI_STORE) {
-        HYMT2_DISPATCH_DTYPE(c_dtype, TC, (launch_pdl(gemm_q8_kernel<EPI_STORE, TC>, grid, dim3(256), 0, stream, p)));
-    } else {
-        HYMT2_REQUIRE(epilogue == EPI_GATED, "gemm_q8_tc: unknown epilogue %d", epilogue);
-        HYMT2_DISPATCH_DTYPE(c_dtype, TC, (launch_pdl(gemm_q8_kernel<EPI_GATED, TC>, grid, dim3(256), 0, stream, p)));
-    }
-    return hymt2_check_launch("gemm_q8_tc");
+    HYMT2_REQUIRE(epilogue >= 0 && epilogue <= 2 && (c_dtype == HYMT2_F32 || (c_dtype == HYMT2_BF16 && epilogue != EPI_ACCUMULATE)),
+                  "gemm_q8_tc: epilogue %d with output type %d is not built", epilogue, c_dtype);
+    HYMT2_REQUIRE(status != nullptr, "gemm_q8_tc: a status word is needed");
+    const Plan pl = make_plan(T, N, K, epilogue == EPI_GATED, sm_count_of_current_device());
+    HYMT2_REQUIRE(pl.tiles_t <= 65535, "gemm_q8_tc: grid too large");
+    const GemmQ8Params p{C, a_scale, w_scale, ldc, T, N, K, pl.bn, pl.stages, pl.splits, pl.k_blocks_per_split, weights_settled, 0, status,
+                         GluRule{glu_kind, glu_limit, glu_alpha, glu_bias}};
+    if (epilogue == EPI_ACCUMULATE) return run<EPI_ACCUMULATE, float>(A, W, lda, ldw, p, pl, stream);
+    if (epilogue == EPI_STORE)
+        return c_dtype == HYMT2_F32 ? run<EPI_STORE, float>(A, W, lda, ldw, p, pl, stream) : run<EPI_STORE, __nv_bfloat16>(A, W, lda, ldw, p, pl, stream);
+    return c_dtype == HYMT2_F32 ? run<EPI_GATED, float>(A, W, lda, ldw, p, pl, stream) : run<EPI_GATED, __nv_bfloat16>(A, W, lda, ldw, p, pl, stream);
 }

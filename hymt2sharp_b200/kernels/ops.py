@@ -41,7 +41,7 @@ _DECLARED = {"hymt2_gemm_tc_norm": "pippiiilllipl" "pippp" "iifppip" "iffp",
              "hymt2_quantize_q8": "plppiliip",
              "hymt2_dequantize_q8": "pilplpiip",
              "hymt2_rmsnorm_q8": "plppilpilplpiiifp",
-             "hymt2_gemm_q8_tc": "pippppiiillli" "pp" "iffp"}
+             "hymt2_gemm_q8_tc": "pippppiiilllii" "pp" "iffp"}
 
 
 def _lib():
@@ -448,7 +448,7 @@ def device_status(device) -> torch.Tensor:
     room for; 3: a position outside the table of positions; 101-106: a wait of the tensor-core GEMM (106: for the partial sums of a tile's other CTAs); 108-119: of the prompt attention; 120-129: of the decode
     attention; 131-139: of the float32 products on tensor cores (131 copies of the weights, 132 pieces and accumulators, 135 stages and buffers to cut into,
     137 sums, 138 and 139 the tokens' pieces); 141-147: of the experts' product of few rows (141 copies, 142 and 145 rows, 143 and 146 accumulators, 144 stages, 147 the
-    quarters' sums))."""
+    quarters' sums); 151-154: of the products of 8-bit integers (151 stages to copy into, 152 copies, 153 sums, 154 drained accumulators))."""
     hit = _status_of.get(device)
     if hit is not None:
         return hit
@@ -2461,10 +2461,11 @@ def rmsnorm_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, gain: torc
 
 
 def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int, status: torch.Tensor,
-               glu: GluRule | None = None, glu_bias: torch.Tensor | None = None) -> None:
+               glu: GluRule | None = None, glu_bias: torch.Tensor | None = None, weights_settled: bool = False) -> None:
     """out[t, n] = epilogue(a_scale[t] * w_scale[n] * sum_k a[t, k] * w[n, k]): 8-bit rows of tokens with 8-bit rows of weights, the sums exact
     in 32-bit integers, the rest in float32.  Store (float32 or bfloat16), accumulate (float32) or SwiGLU (w and w_scale have 2N rows, gates first;
-    `glu` and `glu_bias` as for gemm_tc, with outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row."""
+    `glu` and `glu_bias` as for gemm_tc, with outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row.  `weights_settled`: w was complete before
+    the kernel in front of this call was launched, as a model's weights are; it is then fetched while that one still runs."""
     lda, ldw = _q8(a, a_scale, "a"), _q8(w, w_scale, "w")
     T, K = a.shape
     gated = epilogue == EPILOGUE_SWIGLU
@@ -2486,4 +2487,4 @@ def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: tor
     if T == 0 or N == 0:
         return
     _check(_lib().hymt2_gemm_q8_tc(out.data_ptr(), code, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), T, N, K, lda, ldw, ldo,
-                                   epilogue, status.data_ptr(), _raw_stream(), *rule), "gemm_q8_tc")
+                                   epilogue, 1 if weights_settled else 0, status.data_ptr(), _raw_stream(), *rule), "gemm_q8_tc")
