@@ -16,15 +16,15 @@ struct RowCode {
     bool none;            // zeros: nothing in the row, or nothing that is a number
 };
 
-// `bits`: of the largest |x|, as an unsigned number, which orders infinity and NaN above all others
-__device__ __forceinline__ RowCode row_code(uint32_t bits) {
+// `top`: the largest |x|, infinity and NaN included
+__device__ __forceinline__ RowCode row_code(float top) {
     RowCode c;
-    const float top = __uint_as_float(bits);
-    c.none = bits == 0 || bits >= 0x7f800000u;
+    const bool finite = top < __uint_as_float(0x7f800000u);
+    c.none = !finite || top == 0.f;
     c.f = top > 0x1p100f ? 0x1p-60f : top < 0x1p-60f ? 0x1p90f : 1.0f;
     c.top = top * c.f;
     c.inv = 127.0f / c.top;
-    c.s = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : top / 127.0f;
+    c.s = finite ? top / 127.0f : __uint_as_float(0x7fc00000u);
     return c;
 }
 
@@ -38,45 +38,158 @@ __device__ __noinline__ float q8_settle(float x, float r, float e, float top) {
     const float d = fmaf(-b, top, hi) + lo;
     return d == 0.f ? rintf(b) : d > 0.f ? b + 0.5f : b - 0.5f;
 }
-__device__ __forceinline__ int8_t q8_of(float x, const RowCode& c) {
-    if (c.none) return 0;
-    const float v = x * c.f, t = v * c.inv;
-    float r = rintf(t);
-    if (fabsf(t - r) > NEAR_BORDER) r = q8_settle(v, r, t - r, c.top);
-    return (int8_t)(int)r;
+// x of a row that is all numbers -> the whole number, in the lowest byte.  Adding 1.5 * 2^23 rounds to a whole number (ties to even), whose two's
+// complement then fills the lowest bits.
+constexpr float WHOLE = 12582912.0f;
+template <int V> __device__ __forceinline__ void q8_of(const float (&x)[V], const RowCode& c, uint32_t (&code)[V]) {
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float t = x[i] * c.inv, w = t + WHOLE;
+        code[i] = __float_as_uint(w);
+        near |= fabsf(t - (w - WHOLE)) > NEAR_BORDER;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float t = x[i] * c.inv, r = rintf(t);
+            if (fabsf(t - r) > NEAR_BORDER) code[i] = __float_as_uint(q8_settle(x[i], r, t - r, c.top) + WHOLE);
+        }
+    }
 }
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t pack4(const uint32_t* c) { return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410); }
 
-__device__ __forceinline__ uint32_t block_umax(uint32_t v, uint32_t* scratch) {
-    v = __reduce_max_sync(0xffffffffu, v);
+__device__ __forceinline__ float max_abs(float m, float x) {        // a NaN stays
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+__device__ __forceinline__ float warp_max_bits(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }   // (not negative: as bits)
+
+// A row is held in registers by the threads that share it, CH groups of 8 entries each: WARP = true: a warp a row, several rows a block (up to
+// 1,024 entries: no barrier); else a block a row.  VEC: 8 neighbouring entries a thread, moved 16 bytes at a time; else the threads' entries alternate, so that
+// single ones still move side by side.
+template <bool WARP> struct Place {
+    size_t row;
+    int tid, threads;
+    bool in;
+    __device__ Place(int rows) {
+        if (WARP) { row = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); tid = threadIdx.x & 31; threads = 32; }
+        else { row = blockIdx.x; tid = threadIdx.x; threads = blockDim.x; }
+        in = row < (size_t)rows;
+    }
+};
+
+// the entries [8 (c threads + tid), + 8) (VEC) or c 8 threads + tid, + threads, ... of a row as float32; zeros behind the row's end
+template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* row, int c, int tid, int threads, int width, float (&v)[8]) {
+    if constexpr (VEC) {
+        const int at = 8 * (c * threads + tid);
+        if (at + 8 <= width) {
+            constexpr int N = 16 / sizeof(T);
+#pragma unroll
+            for (int h = 0; h < 8; h += N) {
+                const Pack<T, N> p = load_pack<T, N>(row + at + h);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[h + i] = to_float(p.v[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = at + i < width ? to_float(row[at + i]) : 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int at = (c * 8 + i) * threads + tid;
+            v[i] = at < width ? to_float(row[at]) : 0.f;
+        }
+    }
+}
+template <bool VEC, typename T> __device__ __forceinline__ void store8(T* row, int c, int tid, int threads, int width, const float (&v)[8]) {
+    if constexpr (VEC) {
+        const int at = 8 * (c * threads + tid);
+        if (at + 8 <= width) {
+            constexpr int N = 16 / sizeof(T);
+#pragma unroll
+            for (int h = 0; h < 8; h += N) {
+                Pack<T, N> p;
+#pragma unroll
+                for (int i = 0; i < N; i++) p.v[i] = from_float<T>(v[h + i]);
+                store_pack<T, N>(row + at + h, p);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) if (at + i < width) row[at + i] = from_float<T>(v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int at = (c * 8 + i) * threads + tid;
+            if (at < width) row[at] = from_float<T>(v[i]);
+        }
+    }
+}
+template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* row, int c, int tid, int threads, int width, float (&v)[8], const RowCode& code) {
+    uint32_t w[8];
+    if (code.none) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = 0;
+    } else {
+        if (code.f != 1.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] *= code.f;
+        }
+        q8_of(v, code, w);
+    }
+    if constexpr (VEC) {
+        const int at = 8 * (c * threads + tid);
+        if (at + 8 <= width) *reinterpret_cast<uint2*>(row + at) = make_uint2(pack4(w), pack4(w + 4));
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) if (at + i < width) row[at + i] = (int8_t)w[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int at = (c * 8 + i) * threads + tid;
+            if (at < width) row[at] = (int8_t)w[i];
+        }
+    }
+}
+
+// The largest |x| and (SUM) the sum of the squares over the threads of a row.  Sums in a fixed order.
+template <bool WARP, bool SUM> __device__ __forceinline__ void over_row(float& most, float& ss, float2* scratch) {
+    most = warp_max_bits(most);
+    if (SUM) ss = warp_sum(ss);
+    if (WARP) return;
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) scratch[threadIdx.x >> 5] = make_float2(most, ss);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    for (int w = 0; w < (int)(blockDim.x >> 5); w++) v = max(v, scratch[w]);
-    return v;
+    const float2 mine = lane < warps ? scratch[lane] : make_float2(0.f, 0.f);
+    most = warp_max_bits(mine.x);
+    if (SUM) ss = warp_sum(mine.y);
 }
 
-template <typename TX>
-__global__ void quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int width) {
-    __shared__ uint32_t most_s[32];
-    pdl_wait();
+template <typename TX, int CH, bool WARP, bool VEC>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
+    __shared__ float2 scratch[32];
     pdl_launch_dependents();
-    const size_t r = blockIdx.x;
-    const TX* src = x + r * ldx;
-    uint32_t most = 0;
-    for (int i = threadIdx.x; i < width; i += blockDim.x) most = max(most, abs_bits(to_float(src[i])));
-    const RowCode c = row_code(block_umax(most, most_s));
-    for (int i = threadIdx.x; i < width; i += blockDim.x) q[r * ldq + i] = q8_of(to_float(src[i]), c);
-    if (threadIdx.x == 0) scale[r] = c.s;
-}
-
-template <typename TY>
-__global__ void dequantize_q8_kernel(TY* y, long ldy, const int8_t* q, long ldq, const float* scale, int width) {
     pdl_wait();
-    pdl_launch_dependents();
-    const size_t r = blockIdx.x;
-    const float s = scale[r];
-    for (int i = threadIdx.x; i < width; i += blockDim.x) y[r * ldy + i] = from_float<TY>((float)q[r * ldq + i] * s);
+    const Place<WARP> at(rows);
+    if (!at.in) return;
+    const TX* src = x + at.row * ldx;
+    float v[CH][8], most = 0.f, none = 0.f;
+    // CH loads are in flight before the first is used
+#pragma unroll
+    for (int c = 0; c < CH; c++) load8<VEC>(src, c, at.tid, at.threads, width, v[c]);
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) most = max_abs(most, v[c][i]);
+    over_row<WARP, false>(most, none, scratch);
+    const RowCode code = row_code(most);
+#pragma unroll
+    for (int c = 0; c < CH; c++) store_codes<VEC>(q + at.row * ldq, c, at.tid, at.threads, width, v[c], code);
+    if (at.tid == 0) scale[at.row] = code.s;
 }
 
 struct NormQ8Params {
@@ -86,56 +199,214 @@ struct NormQ8Params {
     void* total;
     const void* gain;
     long ldq, ldx, ldadd, ldt;
-    int width;
+    int rows, width;
     float eps;
 };
 
-template <typename TX, typename TA, typename TG>
-__global__ void rmsnorm_q8_kernel(NormQ8Params p) {
-    __shared__ uint32_t most_s[32];
-    __shared__ float sum_s[33];
-    pdl_wait();
+template <typename TX, typename TA, typename TG, int CH, bool WARP, bool VEC>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_q8_kernel(NormQ8Params p) {
+    __shared__ float2 scratch[32];
     pdl_launch_dependents();
+    pdl_wait();
+    const Place<WARP> at(p.rows);
+    if (!at.in) return;
+    float v[CH][8], most = 0.f, ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; c++) load8<VEC>((const TX*)p.x + at.row * p.ldx, c, at.tid, at.threads, p.width, v[c]);
+    if (p.add) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            float a[8];
+            load8<VEC>((const TA*)p.add + at.row * p.ldadd, c, at.tid, at.threads, p.width, a);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[c][i] = to_float(from_float<TX>(v[c][i] + a[i]));   // the sum as the rows are kept: what is normed is what a later reader finds
+            if (p.total) store8<VEC>((TX*)p.total + at.row * p.ldt, c, at.tid, at.threads, p.width, v[c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        float g[8];
+        load8<VEC>((const TG*)p.gain, c, at.tid, at.threads, p.width, g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            ss = fmaf(v[c][i], v[c][i], ss);
+            v[c][i] *= g[i];
+            most = max_abs(most, v[c][i]);
+        }
+    }
+    over_row<WARP, true>(most, ss, scratch);
+    const RowCode code = row_code(most);
+#pragma unroll
+    for (int c = 0; c < CH; c++) store_codes<VEC>(p.q + at.row * p.ldq, c, at.tid, at.threads, p.width, v[c], code);
+    if (at.tid == 0) p.scale[at.row] = code.s * (1.0f / sqrtf(ss / (float)p.width + p.eps));
+}
+
+// Rows that the registers of 1,024 threads do not hold are read twice, the second time out of L2.
+constexpr int LONGEST_HELD = 16384;
+
+template <typename TX, bool VEC>
+__global__ void __launch_bounds__(1024) quantize_q8_long_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int width) {
+    __shared__ float2 scratch[32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const TX* src = x + (size_t)blockIdx.x * ldx;
+    float most = 0.f, none = 0.f;
+    for (int c = 0; c * 8192 < width; c++) {
+        float v[8];
+        load8<VEC>(src, c, threadIdx.x, 1024, width, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) most = max_abs(most, v[i]);
+    }
+    over_row<false, false>(most, none, scratch);
+    const RowCode code = row_code(most);
+    for (int c = 0; c * 8192 < width; c++) {
+        float v[8];
+        load8<VEC>(src, c, threadIdx.x, 1024, width, v);
+        store_codes<VEC>(q + (size_t)blockIdx.x * ldq, c, threadIdx.x, 1024, width, v, code);
+    }
+    if (threadIdx.x == 0) scale[blockIdx.x] = code.s;
+}
+
+template <typename TX, typename TA, typename TG, bool VEC>
+__global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(NormQ8Params p) {
+    __shared__ float2 scratch[32];
+    pdl_launch_dependents();
+    pdl_wait();
     const size_t r = blockIdx.x;
     const TX* x = (const TX*)p.x + r * p.ldx;
     const TA* add = p.add ? (const TA*)p.add + r * p.ldadd : nullptr;
     TX* total = p.total ? (TX*)p.total + r * p.ldt : nullptr;
-    const TG* gain = (const TG*)p.gain;
-    auto at = [&](int i) { return add ? to_float(from_float<TX>(to_float(x[i]) + to_float(add[i]))) : to_float(x[i]); };
-    uint32_t most = 0;
-    float ss = 0.f;
-    for (int i = threadIdx.x; i < p.width; i += blockDim.x) {
-        const float t = at(i);
-        ss = fmaf(t, t, ss);
-        most = max(most, abs_bits(t * to_float(gain[i])));
+    auto rows_entries = [&](int c, float (&v)[8]) {
+        load8<VEC>(x, c, threadIdx.x, 1024, p.width, v);
+        if (add) {
+            float a[8];
+            load8<VEC>(add, c, threadIdx.x, 1024, p.width, a);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = to_float(from_float<TX>(v[i] + a[i]));
+        }
+    };
+    float v[8], g[8], most = 0.f, ss = 0.f;
+    for (int c = 0; c * 8192 < p.width; c++) {
+        rows_entries(c, v);
+        load8<VEC>((const TG*)p.gain, c, threadIdx.x, 1024, p.width, g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            ss = fmaf(v[i], v[i], ss);
+            most = max_abs(most, v[i] * g[i]);
+        }
     }
-    const RowCode c = row_code(block_umax(most, most_s));
-    const float scale = 1.0f / sqrtf(block_sum(ss, sum_s) / (float)p.width + p.eps);
-    for (int i = threadIdx.x; i < p.width; i += blockDim.x) {
-        const float t = at(i);
-        p.q[r * p.ldq + i] = q8_of(t * to_float(gain[i]), c);
-        if (total) total[i] = from_float<TX>(t);        // (x itself may be the place: entry i is not read again)
+    over_row<false, true>(most, ss, scratch);
+    const RowCode code = row_code(most);
+    for (int c = 0; c * 8192 < p.width; c++) {
+        rows_entries(c, v);
+        if (total) store8<VEC>(total, c, threadIdx.x, 1024, p.width, v);        // (x itself may be the place: these entries are not read again)
+        load8<VEC>((const TG*)p.gain, c, threadIdx.x, 1024, p.width, g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= g[i];
+        store_codes<VEC>(p.q + r * p.ldq, c, threadIdx.x, 1024, p.width, v, code);
     }
-    if (threadIdx.x == 0) p.scale[r] = c.s * scale;
+    if (threadIdx.x == 0) p.scale[r] = code.s * (1.0f / sqrtf(ss / (float)p.width + p.eps));
 }
 
-inline int row_threads(int width) { return width >= 2048 ? 256 : width >= 512 ? 128 : 32; }
+// A warp takes pieces of 4 x 32 groups of 16 output bytes of a row (VEC), or 512 single entries.
+template <typename TY, bool VEC>
+__global__ void __launch_bounds__(256) dequantize_q8_kernel(TY* y, long ldy, const int8_t* q, long ldq, const float* scale, int rows, int width, int pieces) {
+    constexpr int V = VEC ? 16 / (int)sizeof(TY) : 1, STEP = 4 * 32 * V * (VEC ? 1 : 4);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long all = (long)rows * pieces, step = (long)gridDim.x * (blockDim.x >> 5);
+    for (long i = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < all; i += step) {
+        const long r = i / pieces;
+        const int from = (int)(i - r * pieces) * STEP;
+        const int8_t* src = q + r * ldq;
+        TY* dst = y + r * ldy;
+        const float s = scale[r];
+        constexpr int GROUPS = STEP / (32 * V);
+        Pack<int8_t, V> p[GROUPS];
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            const int at = from + (g * 32 + lane) * V;
+            if (at + V <= width) {
+                if constexpr (V == 8) *reinterpret_cast<uint2*>(p[g].v) = *reinterpret_cast<const uint2*>(src + at);
+                else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p[g].v) = *reinterpret_cast<const uint32_t*>(src + at);
+                else p[g].v[0] = src[at];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            const int at = from + (g * 32 + lane) * V;
+            if (at + V <= width) {
+                Pack<TY, V> o;
+#pragma unroll
+                for (int k = 0; k < V; k++) o.v[k] = from_float<TY>((float)p[g].v[k] * s);
+                store_pack<TY, V>(dst + at, o);
+            } else
+                for (int k = at; k < width; k++) dst[k] = from_float<TY>((float)src[k] * s);
+        }
+    }
+}
+
+inline bool whole(const void* p, long ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
+
+// How a row is shared: groups of 8 entries a thread, a warp or a block a row, threads of a block.
+struct Share { int ch, threads, blocks; bool warp; };
+Share share_of(int rows, int width, bool norm) {
+    const int groups = (width + 7) / 8;
+    if (groups <= 128) return Share{groups <= 32 ? 1 : groups <= 64 ? 2 : 4, 256, (rows + 7) / 8, true};
+    // (a norm's sums are added in an order that the share decides, so its share hangs on the width alone)
+    const int ch = norm && groups <= 1024 ? 1 : 2;
+    return Share{ch, ((groups + ch - 1) / ch + 31) / 32 * 32, rows, false};
+}
+
+template <typename TX, bool VEC>
+int run_quantize(const Share& s, int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width, cudaStream_t stream) {
+#define HYMT2_RUN(CH, WARP) launch_pdl(quantize_q8_kernel<TX, CH, WARP, VEC>, dim3(s.blocks), dim3(s.threads), 0, stream, q, ldq, scale, x, ldx, rows, width)
+    if (s.warp) s.ch == 1 ? HYMT2_RUN(1, true) : s.ch == 2 ? HYMT2_RUN(2, true) : HYMT2_RUN(4, true);
+    else HYMT2_RUN(2, false);
+#undef HYMT2_RUN
+    return hymt2_check_launch("quantize_q8");
+}
+template <typename TX, typename TA, typename TG, bool VEC>
+int run_norm(const Share& s, const NormQ8Params& p, cudaStream_t stream) {
+#define HYMT2_RUN(CH, WARP) launch_pdl(rmsnorm_q8_kernel<TX, TA, TG, CH, WARP, VEC>, dim3(s.blocks), dim3(s.threads), 0, stream, p)
+    if (s.warp) s.ch == 1 ? HYMT2_RUN(1, true) : s.ch == 2 ? HYMT2_RUN(2, true) : HYMT2_RUN(4, true);
+    else s.ch == 1 ? HYMT2_RUN(1, false) : HYMT2_RUN(2, false);
+#undef HYMT2_RUN
+    return hymt2_check_launch("rmsnorm_q8");
+}
 
 }  // namespace
 
 HYMT2_API int hymt2_quantize_q8(void* q, long ldq, float* scale, const void* x, int x_dtype, long ldx, int rows, int width, cudaStream_t stream) {
     if (rows == 0) return HYMT2_OK;
     HYMT2_REQUIRE(rows > 0 && width > 0 && ldq >= width && ldx >= width, "quantize_q8: bad sizes rows=%d width=%d", rows, width);
-    HYMT2_DISPATCH_DTYPE(x_dtype, TX, (launch_pdl(quantize_q8_kernel<TX>, dim3(rows), dim3(row_threads(width)), 0, stream, (int8_t*)q, ldq, scale,
-                                                  (const TX*)x, ldx, width)));
-    return hymt2_check_launch("quantize_q8");
+    HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "quantize_q8: rows of integers must start on 16 bytes");
+    HYMT2_DISPATCH_DTYPE(x_dtype, TX, {
+        if (width > LONGEST_HELD) {
+            launch_pdl(whole(x, ldx, sizeof(TX)) ? quantize_q8_long_kernel<TX, true> : quantize_q8_long_kernel<TX, false>, dim3(rows), dim3(1024), 0, stream,
+                       (int8_t*)q, ldq, scale, (const TX*)x, ldx, width);
+            return hymt2_check_launch("quantize_q8");
+        }
+        const Share s = share_of(rows, width, false);
+        if (whole(x, ldx, sizeof(TX))) return run_quantize<TX, true>(s, (int8_t*)q, ldq, scale, (const TX*)x, ldx, rows, width, stream);
+        return run_quantize<TX, false>(s, (int8_t*)q, ldq, scale, (const TX*)x, ldx, rows, width, stream);
+    });
 }
 
 HYMT2_API int hymt2_dequantize_q8(void* y, int y_dtype, long ldy, const void* q, long ldq, const float* scale, int rows, int width, cudaStream_t stream) {
     if (rows == 0) return HYMT2_OK;
     HYMT2_REQUIRE(rows > 0 && width > 0 && ldq >= width && ldy >= width, "dequantize_q8: bad sizes rows=%d width=%d", rows, width);
-    HYMT2_DISPATCH_DTYPE(y_dtype, TY, (launch_pdl(dequantize_q8_kernel<TY>, dim3(rows), dim3(row_threads(width)), 0, stream, (TY*)y, ldy,
-                                                  (const int8_t*)q, ldq, scale, width)));
+    HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "dequantize_q8: rows of integers must start on 16 bytes");
+    HYMT2_DISPATCH_DTYPE(y_dtype, TY, {
+        const bool vec = whole(y, ldy, sizeof(TY));
+        const int step = vec ? 2048 / (int)sizeof(TY) : 512, pieces = (width + step - 1) / step;
+        const long warps = (long)rows * pieces;
+        const long blocks = (warps + 7) / 8;
+        const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+        if (vec) launch_pdl(dequantize_q8_kernel<TY, true>, grid, dim3(256), 0, stream, (TY*)y, ldy, (const int8_t*)q, ldq, scale, rows, width, pieces);
+        else launch_pdl(dequantize_q8_kernel<TY, false>, grid, dim3(256), 0, stream, (TY*)y, ldy, (const int8_t*)q, ldq, scale, rows, width, pieces);
+    });
     return hymt2_check_launch("dequantize_q8");
 }
 
@@ -144,9 +415,17 @@ HYMT2_API int hymt2_rmsnorm_q8(void* q, long ldq, float* scale, const void* x, i
                                void* total, long ldt, const void* gain, int gain_dtype, int rows, int width, float eps, cudaStream_t stream) {
     if (rows == 0) return HYMT2_OK;
     HYMT2_REQUIRE(rows > 0 && width > 0 && ldq >= width && ldx >= width, "rmsnorm_q8: bad sizes rows=%d width=%d", rows, width);
+    HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "rmsnorm_q8: rows of integers must start on 16 bytes");
     HYMT2_REQUIRE(!total || add, "rmsnorm_q8: the sums have a place, but nothing is added");
-    const NormQ8Params p{(int8_t*)q, scale, x, add, total, gain, ldq, ldx, ldadd, ldt, width, eps};
-    HYMT2_DISPATCH_DTYPE(x_dtype, TX, HYMT2_DISPATCH_DTYPE(add_dtype, TA, HYMT2_DISPATCH_DTYPE(gain_dtype, TG,
-        (launch_pdl(rmsnorm_q8_kernel<TX, TA, TG>, dim3(rows), dim3(row_threads(width)), 0, stream, p)))));
-    return hymt2_check_launch("rmsnorm_q8");
+    const NormQ8Params p{(int8_t*)q, scale, x, add, total, gain, ldq, ldx, ldadd, ldt, rows, width, eps};
+    const Share s = share_of(rows, width, true);
+    HYMT2_DISPATCH_DTYPE(x_dtype, TX, HYMT2_DISPATCH_DTYPE(add_dtype, TA, HYMT2_DISPATCH_DTYPE(gain_dtype, TG, {
+        const bool vec = whole(x, ldx, sizeof(TX)) && (!add || whole(add, ldadd, sizeof(TA))) && (!total || whole(total, ldt, sizeof(TX))) &&
+                         (uintptr_t)gain % 16 == 0;
+        if (width > LONGEST_HELD) {
+            launch_pdl(vec ? rmsnorm_q8_long_kernel<TX, TA, TG, true> : rmsnorm_q8_long_kernel<TX, TA, TG, false>, dim3(rows), dim3(1024), 0, stream, p);
+            return hymt2_check_launch("rmsnorm_q8");
+        }
+        return vec ? run_norm<TX, TA, TG, true>(s, p, stream) : run_norm<TX, TA, TG, false>(s, p, stream);
+    })));
 }
