@@ -12,10 +12,12 @@
 // Rows, tokens and K beyond the matrices are zeros by TMA and masked in the epilogue.  Every wait on an mbarrier is bounded (see tc_common.cuh).
 #include "tc_common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 enum { EPI_STORE = 0, EPI_ACCUMULATE = 1, EPI_GATED = 2 };
-constexpr int MAX_K = 131071, BLOCK_K = 128, UMMA_K = 32, TILE_M = 128, MAX_STAGES = 8;
+constexpr int MAX_K = 131071, BLOCK_K = 128, UMMA_K = 32, TILE_M = 128, MAX_STAGES = 12;
 constexpr int A_TILE_BYTES = TILE_M * BLOCK_K;
 // instruction descriptor: D 32-bit integers, A and B signed 8-bit integers, both K-major
 __host__ __device__ constexpr uint32_t idesc_q8(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
@@ -42,13 +44,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// x sigmoid(alpha x) by the hardware's approximate exponential and reciprocal (together within 2^-22 of the result and 2^-24 of the exponent's size): an exact
+// division and exponential took the drain of a gated tile three times as long as its MMAs (2,048 x 6,144 gated x 2,048: 74 against 40 us).
+__device__ __forceinline__ float swish(float x, float alpha) {
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-alpha * x)));
+    return x * r;
+}
 // glu_at of common.cuh, but a NaN stays one under the clamps: it says that the row held one before it became integers
 __device__ __forceinline__ float gated_at(const GluRule& r, float g, float u, int n, int N) {
     if (r.bias) { g = __fadd_rn(g, r.bias[n]); u = __fadd_rn(u, r.bias[N + n]); }
-    if (r.kind == GLU_SILU) return silu_mul(g, u);
+    if (r.kind == GLU_SILU) return swish(g, 1.0f) * u;
     g = min_nan(g, r.limit);
     u = min_nan(max_nan(u, -r.limit), r.limit);
-    return g / (1.0f + expf(-r.alpha * g)) * (u + 1.0f);
+    return swish(g, r.alpha) * (u + 1.0f);
 }
 // (products of their own and no FMA with what follows: both kernels give the same bits)
 __device__ __forceinline__ float scaled(int sum, float a, float w) { return __fmul_rn(__fmul_rn((float)sum, a), w); }
@@ -80,6 +89,39 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void mbar_arrive_even(uint32_t even_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_bar) : "memory");
 }
+// A look at a barrier that does not wait.  The roles look at the next stage's barrier in front of this stage's work, so that the answer's way (a
+// few hundred cycles under load) passes behind that work, and wait only where the look saw nothing.
+__device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A warp reads N columns from each of two places of its 32 lanes of tensor memory, one row a thread.
+template <int N> __device__ __forceinline__ void tmem_load_two(uint32_t at_a, uint32_t at_b, float* a, float* b);
+template <> __device__ __forceinline__ void tmem_load_two<16>(uint32_t at_a, uint32_t at_b, float* a, float* b) {
+    uint32_t *r = reinterpret_cast<uint32_t*>(a), *q = reinterpret_cast<uint32_t*>(b);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15])
+        : "r"(at_a), "r"(at_b) : "memory");
+}
+template <> __device__ __forceinline__ void tmem_load_two<32>(uint32_t at_a, uint32_t at_b, float* a, float* b) {
+    uint32_t *r = reinterpret_cast<uint32_t*>(a), *q = reinterpret_cast<uint32_t*>(b);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]), "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]), "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+        : "r"(at_a), "r"(at_b) : "memory");
+}
 __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t local_addr, uint32_t rank) {
     const float4 v = ld_cluster_f32x4(local_addr, rank);
     return make_int4(__float_as_int(v.x), __float_as_int(v.y), __float_as_int(v.z), __float_as_int(v.w));
@@ -88,11 +130,11 @@ __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t local_addr, uint32_t r
 // --------------------------------------------------------------------------------------------
 // Few tokens: a CTA computes 128 weight rows (gated: 128 gate and 128 up rows) x BN tokens over its cut of K.
 // --------------------------------------------------------------------------------------------
-constexpr int FEW_THREADS = 192;       // warp 0 TMA, warp 1 MMAs, warps 2 to 5 the sums
+__host__ __device__ constexpr int few_warps(int bn) { return bn >= 64 ? 8 : 4; }      // that drain the sums (behind warp 0, TMA, and warp 1, MMAs)
 constexpr int MAX_RANKS = 8;           // a portable cluster
 
 template <int BN, int EPI, typename TC>
-__global__ void __launch_bounds__(FEW_THREADS)
+__global__ void __launch_bounds__(64 + 32 * few_warps(BN))
 gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, GemmQ8Params p) {
     constexpr int NUM_ACC = EPI == EPI_GATED ? 2 : 1;
     constexpr int STAGE_BYTES = NUM_ACC * A_TILE_BYTES + BN * BLOCK_K;
@@ -166,17 +208,21 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         constexpr uint64_t K_STEP = UMMA_K >> 4, A2_STEP = A_TILE_BYTES >> 4, B_STEP = (NUM_ACC * A_TILE_BYTES) >> 4;
         const uint64_t desc0 = desc_k_major(tiles);
         uint32_t s = 0, phase = 0;
+        bool seen = false;
         for (int i = 0; i < my_blocks; i++) {
-            if (!mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152)) break;
+            if (!seen && !mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t adesc = desc0 + (uint64_t)s * (uint64_t)(STAGE_BYTES >> 4), bdesc = adesc + B_STEP;
+            const uint32_t s_next = s + 1 == (uint32_t)stages ? 0 : s + 1, phase_next = s_next ? phase : phase ^ 1;
+            seen = mbar_look(full0 + 8 * s_next, phase_next);       // (behind the last block nothing comes of it)
 #pragma unroll
             for (int k = 0; k < BLOCK_K / UMMA_K; k++) {
                 umma_q8(tmem_base, adesc + k * K_STEP, bdesc + k * K_STEP, IDESC, i > 0 || k > 0);
                 if (NUM_ACC == 2) umma_q8(tmem_base + BN, adesc + A2_STEP + k * K_STEP, bdesc + k * K_STEP, IDESC, i > 0 || k > 0);
             }
             umma_commit(empty0 + 8 * s);
-            if (++s == (uint32_t)stages) { s = 0; phase ^= 1; }
+            s = s_next;
+            phase = phase_next;
         }
         umma_commit(done_bar);
     } else if (warp >= 2) {
@@ -198,11 +244,12 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // the sums -> this CTA's shared memory (the ring is free now), [column][row]
-        constexpr int CH = BN >= 32 ? 32 : 16;
+        constexpr int CH = BN >= 32 ? 32 : 16, GROUPS = few_warps(BN) / 4;
+        const int group = (warp - 2) >> 2;
 #pragma unroll 1
         for (int h = 0; h < NUM_ACC; h++)
 #pragma unroll 1
-            for (int c = 0; c < cols; c += CH) {
+            for (int c = group * CH; c < cols; c += GROUPS * CH) {
                 float g[CH];
                 if (ok && my_blocks > 0) {
                     if constexpr (CH == 32) tmem_load32(lane_addr + h * BN + c, g);
@@ -217,51 +264,78 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
         __syncwarp();
         if (p.splits > 1) cluster_sync_all();
-        else asm volatile("bar.sync 1, 128;" ::: "memory");
-        // every CTA of the cluster takes a share of the tokens, adds all ranks' sums for them and writes them out; a warp has a token,
-        // a lane four weight rows
+        else asm volatile("bar.sync 1, %0;" ::"n"(32 * few_warps(BN)) : "memory");
+        // every CTA of the cluster takes a share of the tokens, adds all ranks' sums for them and writes them out; a warp has a token, a lane four
+        // weight rows.  The way to another CTA's memory is long (one token at a time took 170 ns a token), so the sums of U tokens and R ranks are
+        // asked for together: many tokens a warp where there are few ranks, and the other way round.
+        constexpr int WARPS = few_warps(BN);
         const int share = (cols + p.splits - 1) / p.splits;
         const int c_begin = (int)blockIdx.z * share, c_end = min(cols, c_begin + share);
+        auto fold = [&](auto tokens, auto ranks) {
+            constexpr int U = decltype(tokens)::value, R = decltype(ranks)::value;
 #pragma unroll 1
-        for (int c = c_begin + quarter; c < c_end; c += 4) {
-            int4 part[NUM_ACC][MAX_RANKS];
+            for (int c0 = c_begin + warp - 2; c0 < c_end; c0 += WARPS * U) {
+                int4 part[U][R][NUM_ACC];
+                float sa[U];
 #pragma unroll
-            for (int r = 0; r < MAX_RANKS; r++)
+                for (int k = 0; k < U; k++) {
+                    const int c = c0 + k * WARPS;
+                    sa[k] = c < c_end ? p.a_scale[t0 + c] : 0.f;
 #pragma unroll
-                for (int h = 0; h < NUM_ACC; h++)
-                    part[h][r] = r < p.splits ? ld_cluster_s32x4(tiles + ((h * BN + c) * TILE_M + 4 * lane) * 4, r) : make_int4(0, 0, 0, 0);
-            const float sa = p.a_scale[t0 + c];
-            float y[NUM_ACC][4];
+                    for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int h = 0; h < NUM_ACC; h++) {
-                int4 sum = part[h][0];
-#pragma unroll
-                for (int r = 1; r < MAX_RANKS; r++) { sum.x += part[h][r].x; sum.y += part[h][r].y; sum.z += part[h][r].z; sum.w += part[h][r].w; }
-                y[h][0] = scaled(sum.x, sa, sw[h][0]); y[h][1] = scaled(sum.y, sa, sw[h][1]);
-                y[h][2] = scaled(sum.z, sa, sw[h][2]); y[h][3] = scaled(sum.w, sa, sw[h][3]);
-            }
-            TC* dst = C + (size_t)(t0 + c) * p.ldc + n4;
-            if constexpr (EPI == EPI_GATED) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) if (n4 + i < p.N) y[0][i] = gated_at(p.glu, y[0][i], y[1][i], n4 + i, p.N);
-            }
-            if (vec) {
-                if constexpr (EPI == EPI_ACCUMULATE) {
-                    const float4 old = *reinterpret_cast<const float4*>(dst);
-                    y[0][0] = __fadd_rn(old.x, y[0][0]); y[0][1] = __fadd_rn(old.y, y[0][1]);
-                    y[0][2] = __fadd_rn(old.z, y[0][2]); y[0][3] = __fadd_rn(old.w, y[0][3]);
+                        for (int h = 0; h < NUM_ACC; h++) {
+                            const uint32_t at = tiles + ((h * BN + c) * TILE_M + 4 * lane) * 4;
+                            part[k][r][h] = make_int4(0, 0, 0, 0);
+                            if (c < c_end && r < p.splits) {
+                                if constexpr (R == 1)
+                                    asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(part[k][r][h].x), "=r"(part[k][r][h].y),
+                                                 "=r"(part[k][r][h].z), "=r"(part[k][r][h].w) : "r"(at) : "memory");
+                                else part[k][r][h] = ld_cluster_s32x4(at, r);
+                            }
+                        }
                 }
-                if constexpr (sizeof(TC) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0][0], y[0][1], y[0][2], y[0][3]);
-                else {
-                    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(y[0][0], y[0][1]), __floats2bfloat162_rn(y[0][2], y[0][3])};
-                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
-                }
-            } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (n4 + i < p.N) dst[i] = from_float<TC>(EPI == EPI_ACCUMULATE ? __fadd_rn(to_float(dst[i]), y[0][i]) : y[0][i]);
+                for (int k = 0; k < U; k++) {
+                    const int c = c0 + k * WARPS;
+                    if (c >= c_end) break;
+                    float y[NUM_ACC][4];
+#pragma unroll
+                    for (int h = 0; h < NUM_ACC; h++) {
+                        int4 sum = part[k][0][h];
+#pragma unroll
+                        for (int r = 1; r < R; r++) { sum.x += part[k][r][h].x; sum.y += part[k][r][h].y; sum.z += part[k][r][h].z; sum.w += part[k][r][h].w; }
+                        y[h][0] = scaled(sum.x, sa[k], sw[h][0]); y[h][1] = scaled(sum.y, sa[k], sw[h][1]);
+                        y[h][2] = scaled(sum.z, sa[k], sw[h][2]); y[h][3] = scaled(sum.w, sa[k], sw[h][3]);
+                    }
+                    TC* dst = C + (size_t)(t0 + c) * p.ldc + n4;
+                    if constexpr (EPI == EPI_GATED) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) if (n4 + i < p.N) y[0][i] = gated_at(p.glu, y[0][i], y[1][i], n4 + i, p.N);
+                    }
+                    if (vec) {
+                        if constexpr (EPI == EPI_ACCUMULATE) {
+                            const float4 old = *reinterpret_cast<const float4*>(dst);
+                            y[0][0] = __fadd_rn(old.x, y[0][0]); y[0][1] = __fadd_rn(old.y, y[0][1]);
+                            y[0][2] = __fadd_rn(old.z, y[0][2]); y[0][3] = __fadd_rn(old.w, y[0][3]);
+                        }
+                        if constexpr (sizeof(TC) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0][0], y[0][1], y[0][2], y[0][3]);
+                        else {
+                            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(y[0][0], y[0][1]), __floats2bfloat162_rn(y[0][2], y[0][3])};
+                            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (n4 + i < p.N) dst[i] = from_float<TC>(EPI == EPI_ACCUMULATE ? __fadd_rn(to_float(dst[i]), y[0][i]) : y[0][i]);
+                    }
+                }
             }
-        }
+        };
+        if (p.splits == 1) fold(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+        else if (p.splits == 2) fold(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+        else if (p.splits <= 4) fold(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+        else fold(std::integral_constant<int, 1>{}, std::integral_constant<int, MAX_RANKS>{});
         __syncwarp();
     }
     if (p.splits > 1) {         // no CTA leaves before its peers have read its sums; the other warps come to both barriers too
@@ -334,21 +408,24 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     if (warp == 0 && elect_one()) {
         uint32_t s = 0, round = 0;
         const uint32_t even_full0 = at_rank(full0, 0);
-        bool first = true;
+        bool first = true, seen = false;
         if (!p.early) pdl_wait();
         for (int tile = pair; tile < num_tiles && !*abort_flag; tile += pairs) {
             const int a_row = (tile % tiles_t) * 2 * TILE_M + rank * TILE_M;
             // the even CTA brings the first half of the weight rows, the odd one the second; of gated rows the gates and the ups
             const int w_row = (tile / tiles_t) * OUT_COLS + rank * (GATED ? p.N : bn / 2);
             for (int kb = 0; kb < num_k_blocks; kb++) {
-                if (round > 0 && !mbar_wait(empty0 + 8 * s, (round & 1) ^ 1, abort_flag, p.status, 151)) break;
+                if (round > 0 && !seen && !mbar_wait(empty0 + 8 * s, (round & 1) ^ 1, abort_flag, p.status, 151)) break;
                 const uint32_t bar = even_full0 + 8 * s, a_dst = tiles + s * STAGE_BYTES;
+                const uint32_t s_next = s + 1 == (uint32_t)stages ? 0 : s + 1, round_next = s_next ? round : round + 1;
+                seen = round_next > 0 && mbar_look(empty0 + 8 * s_next, (round_next & 1) ^ 1);
                 if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
                 tma_load_2d_pair(a_dst + A_TILE_BYTES, &map_w, bar, kb * BLOCK_K, w_row);
                 if (first && p.early) pdl_wait();
                 first = false;
                 tma_load_2d_pair(a_dst, &map_a, bar, kb * BLOCK_K, a_row);
-                if (++s == (uint32_t)stages) { s = 0; round++; }
+                s = s_next;
+                round = round_next;
             }
         }
         if (rank == 0 && *abort_flag)   // copies in flight (both CTAs' are counted here) must land before the shared memory goes away
@@ -360,6 +437,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     } else if (warp == 1 && rank == 0 && elect_one()) {
         const uint64_t desc0 = desc_k_major(tiles);
         uint32_t s = 0, phase = 0;
+        bool seen = false;
         int j = 0;
         for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
             const int buf = j & 1;
@@ -367,14 +445,17 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             bool ok = true;
             for (int kb = 0; kb < num_k_blocks; kb++) {
-                if (!(ok = mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152))) break;
+                if (!seen && !(ok = mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t adesc = desc0 + (uint64_t)s * (uint64_t)(STAGE_BYTES >> 4), bdesc = adesc + (A_TILE_BYTES >> 4);
+                const uint32_t s_next = s + 1 == (uint32_t)stages ? 0 : s + 1, phase_next = s_next ? phase : phase ^ 1;
+                seen = mbar_look(full0 + 8 * s_next, phase_next);
 #pragma unroll
                 for (int k = 0; k < BLOCK_K / UMMA_K; k++)
                     umma_q8_pair(tmem_base + buf * PAIR_BN, adesc + k * (UMMA_K >> 4), bdesc + k * (UMMA_K >> 4), IDESC, kb > 0 || k > 0);
                 umma_pair_commit(empty0 + 8 * s);
-                if (++s == (uint32_t)stages) { s = 0; phase ^= 1; }
+                s = s_next;
+                phase = phase_next;
             }
             if (!ok) break;
             umma_pair_commit(acc_full0 + 8 * buf);
@@ -384,12 +465,28 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const uint32_t stage_out = tiles + stages * STAGE_BYTES + (warp - 2) * 2 * OUT_BUFFER;
         pdl_wait();             // C may still be in use by the kernel in front, and the scales come from it
         TC* C = (TC*)p.C;
+        const bool plain = p.glu.kind == GLU_SILU && !p.glu.bias;
         int j = 0, used = 0;
+        // the token's scale, and the scale of one column of a piece a lane (gated: of its gate and its up row): fetched a tile and a piece ahead
+        auto first_token = [&](int tile) { return (tile % tiles_t) * 2 * TILE_M + rank * TILE_M + quarter * 32; };
+        auto token_scale = [&](int tile) {
+            const int t = first_token(tile) + lane;
+            return tile < num_tiles && t < p.T ? __ldg(p.a_scale + t) : 0.f;
+        };
+        auto column_scale = [&](int tile, int c, int h) {
+            const int n = (tile / tiles_t) * OUT_COLS + c + lane;
+            return tile < num_tiles && c < OUT_COLS && lane < PIECE && n < p.N ? __ldg(p.w_scale + (size_t)h * p.N + n) : 0.f;
+        };
+        float sa_next = token_scale(pair), ws_next = column_scale(pair, side * PIECE, 0), us_next = GATED ? column_scale(pair, side * PIECE, 1) : 0.f;
         for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
             const int buf = j & 1;
-            const int t_first = (tile % tiles_t) * 2 * TILE_M + rank * TILE_M + quarter * 32, t = t_first + lane;
+            const int t_first = first_token(tile), t = t_first + lane;
             const int n_first = (tile / tiles_t) * OUT_COLS;
-            const float sa = t < p.T ? p.a_scale[t] : 0.f;
+            const float sa = sa_next;
+            float ws = ws_next, us = us_next;
+            sa_next = token_scale(tile + pairs);
+            ws_next = column_scale(tile + pairs, side * PIECE, 0);
+            if constexpr (GATED) us_next = column_scale(tile + pairs, side * PIECE, 1);
             const bool landed = mbar_wait(acc_full0 + 8 * buf, (uint32_t)((j >> 1) & 1), abort_flag, p.status, 153);
             if (!__all_sync(0xffffffffu, landed)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -399,31 +496,24 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 const int n = n_first + c;
                 if (n >= p.N || t_first >= p.T) break;               // (the same for the whole warp)
                 float y[PIECE], u[GATED ? PIECE : 1];
-                if constexpr (PIECE == 32) {
-                    tmem_load32(lane_addr + c, y);
-                    if constexpr (GATED) tmem_load32(lane_addr + bn / 2 + c, u);
-                } else {
-                    tmem_load16(lane_addr + c, y);
-                    if constexpr (GATED) tmem_load16(lane_addr + bn / 2 + c, u);
-                }
-                auto scale_all = [&](float* v, const float* w) {
-                    if (n + PIECE <= p.N && (uintptr_t)w % 16 == 0) {
+                if constexpr (GATED) tmem_load_two<PIECE>(lane_addr + c, lane_addr + bn / 2 + c, y, u);
+                else if constexpr (PIECE == 32) tmem_load32(lane_addr + c, y);
+                else tmem_load16(lane_addr + c, y);
+                const float ws_now = ws, us_now = us;
+                ws = column_scale(tile, c + 2 * PIECE, 0);
+                if constexpr (GATED) us = column_scale(tile, c + 2 * PIECE, 1);
 #pragma unroll
-                        for (int q = 0; q < PIECE; q += 4) {
-                            const float4 s4 = __ldg(reinterpret_cast<const float4*>(w + q));
-                            v[q] = scaled(__float_as_int(v[q]), sa, s4.x); v[q + 1] = scaled(__float_as_int(v[q + 1]), sa, s4.y);
-                            v[q + 2] = scaled(__float_as_int(v[q + 2]), sa, s4.z); v[q + 3] = scaled(__float_as_int(v[q + 3]), sa, s4.w);
-                        }
+                for (int q = 0; q < PIECE; q++) y[q] = scaled(__float_as_int(y[q]), sa, __shfl_sync(0xffffffffu, ws_now, q));
+                if constexpr (GATED) {
+#pragma unroll
+                    for (int q = 0; q < PIECE; q++) u[q] = scaled(__float_as_int(u[q]), sa, __shfl_sync(0xffffffffu, us_now, q));
+                    if (plain) {
+#pragma unroll
+                        for (int q = 0; q < PIECE; q++) y[q] = swish(y[q], 1.0f) * u[q];
                     } else {
 #pragma unroll
-                        for (int q = 0; q < PIECE; q++) v[q] = scaled(__float_as_int(v[q]), sa, n + q < p.N ? __ldg(w + q) : 0.f);
+                        for (int q = 0; q < PIECE; q++) y[q] = n + q < p.N ? gated_at(p.glu, y[q], u[q], n + q, p.N) : 0.f;
                     }
-                };
-                scale_all(y, p.w_scale + n);
-                if constexpr (GATED) {
-                    scale_all(u, p.w_scale + (size_t)p.N + n);
-#pragma unroll
-                    for (int q = 0; q < PIECE; q++) y[q] = n + q < p.N ? gated_at(p.glu, y[q], u[q], n + q, p.N) : 0.f;
                 }
                 if (p.tma_out) {
                     // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them; the buffer of two pieces ago has been read
@@ -510,46 +600,86 @@ struct Plan {
     int bn, stages, splits, k_blocks_per_split;
     int tiles_n, tiles_t, ctas;
     size_t smem;
+    double cost;             // ns
 };
 
-Plan make_plan(int T, int N, int K, bool gated, int sm_count) {
-    Plan pl{};
+// What decides between the kernels, widths and cuts: estimates of a call's time in ns, fitted to sweeps of 1 to 6,000 tokens over eleven weights of 1,000 x 500
+// to 28,672 x 4,096 with every width and cut.  The rule's choice was within 4 % of the best one at 147 of 187 products and within 15 % at all others but two.
+// A CTA of the few-token kernel takes 200 ns a k block as long as its SM takes in less than 145 bytes a ns; partial sums cost by the number of ranks, and more
+// where more tokens are folded.  A pair by itself takes 1.07 ns a k block and weight row, and no less than its tiles' way from L2 (165 ns); with all SMs at
+// work (power, L2) 115 ns and 0.76 ns a weight row.
+constexpr double BYTES_NS = 6500.0, SM_BYTES_NS = 145.0, FEW_BLOCK_NS = 200.0, PAIR_BLOCK_NS = 165.0, PAIR_COLUMN_NS = 1.07, PAIR_BUSY_NS = 115.0,
+                 PAIR_BUSY_COLUMN_NS = 0.76, PAIR_TILE_NS = 600.0;
+
+// clusters of c CTAs lie inside one GPC, whose SMs they seldom fill: the CTAs that are on the device at one time with one on an SM (of 148)
+constexpr int RESIDENT[MAX_RANKS] = {148, 144, 132, 128, 120, 104, 104, 104};
+
+bool plan_few(Plan& pl, int T, int N, int K, bool gated, int sm_count, int bn, int want) {
     const int k_blocks = (K + BLOCK_K - 1) / BLOCK_K;
-    pl.few = T <= 128;
+    pl.few = true;
+    pl.bn = bn;
+    pl.tiles_n = (N + TILE_M - 1) / TILE_M;
+    pl.tiles_t = (T + bn - 1) / bn;
+    pl.k_blocks_per_split = (k_blocks + want - 1) / want;
+    pl.splits = (k_blocks + pl.k_blocks_per_split - 1) / pl.k_blocks_per_split;
+    if (want > 1 && (pl.splits != want || pl.k_blocks_per_split < 2)) return false;
+    const long ctas = (long)pl.tiles_n * pl.tiles_t * pl.splits, one = (long)RESIDENT[pl.splits - 1] * sm_count / 148;
+    if (pl.splits > 1 && ctas > 2 * one) return false;       // a second wave of clusters costs a call's whole latency again
+    if (pl.tiles_t > 65535 || ctas > 2147483647L) return false;
+    pl.ctas = (int)ctas;
+    const int acc = gated ? 2 : 1, stage = acc * A_TILE_BYTES + bn * BLOCK_K, sums = acc * bn * TILE_M * 4;
+    int stages = (ctas <= one ? 200 : 110) * 1024 / stage;     // an SM's whole memory, or half where two CTAs share one
+    stages = stages > MAX_STAGES ? MAX_STAGES : stages > pl.k_blocks_per_split ? pl.k_blocks_per_split : stages;
+    pl.stages = stages < 2 ? 2 : stages;
+    const size_t ring = (size_t)pl.stages * stage;
+    pl.smem = (ring > (size_t)sums ? ring : (size_t)sums) + 1024;
+    const double on_sm = ctas <= one ? 1 : pl.splits > 1 ? 2 : (double)((ctas + sm_count - 1) / sm_count);
+    const double block = stage / SM_BYTES_NS * on_sm > FEW_BLOCK_NS ? stage / SM_BYTES_NS * on_sm : FEW_BLOCK_NS;
+    const double memory = ((double)acc * N * K + (double)T * K) / BYTES_NS, stream = pl.k_blocks_per_split * block + (memory < 4000 ? 0.5 * memory : 2000.0);
+    const int columns = T < bn ? T : bn;
+    const double start = bn <= 32 ? (gated ? 3900 : 3400) : (gated ? 5600 : 3600) + (columns > 64 ? (columns - 64) * (gated ? 50.0 : 20.0) : 0.0);
+    const double waves = pl.splits == 1 && ctas > one ? (double)ctas / one : 1.0, tokens = 100.0 * (pl.tiles_t - 1);
+    const double fold = (pl.splits - 1) * (bn == 16 ? 100.0 : bn == 32 ? 200.0 : 450.0);
+    pl.cost = start * waves + tokens + fold + (stream > memory ? stream : memory);
+    return true;
+}
+
+void plan_pairs(Plan& pl, int T, int N, int K, bool gated, int sm_count, int bn) {
+    const int k_blocks = (K + BLOCK_K - 1) / BLOCK_K, out = gated ? bn / 2 : bn, pairs = sm_count / 2;
+    pl.few = false;
+    pl.bn = bn;
     pl.splits = 1;
     pl.k_blocks_per_split = k_blocks;
-    if (pl.few) {
-        pl.bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-        pl.tiles_n = (N + TILE_M - 1) / TILE_M;
-        pl.tiles_t = (T + pl.bn - 1) / pl.bn;
-        const int tiles = pl.tiles_n * pl.tiles_t;
-        int want = 2 * sm_count / tiles;
-        want = want < 1 ? 1 : want > MAX_RANKS ? MAX_RANKS : want;
-        while (want > 1 && k_blocks / want < 2) want--;
-        pl.k_blocks_per_split = (k_blocks + want - 1) / want;
-        pl.splits = (k_blocks + pl.k_blocks_per_split - 1) / pl.k_blocks_per_split;
-        pl.ctas = tiles * pl.splits;
-        const int stage = (gated ? 2 : 1) * A_TILE_BYTES + pl.bn * BLOCK_K, sums = (gated ? 2 : 1) * pl.bn * TILE_M * 4;
-        int stages = 110 * 1024 / stage;
-        stages = stages > MAX_STAGES ? MAX_STAGES : stages;
-        stages = stages > pl.k_blocks_per_split ? pl.k_blocks_per_split : stages;
-        pl.stages = stages < 2 ? 2 : stages;
-        const size_t ring = (size_t)pl.stages * stage;
-        pl.smem = (ring > (size_t)sums ? ring : (size_t)sums) + 1024;
-        return pl;
-    }
-    pl.bn = PAIR_BN;
-    const int out = gated ? pl.bn / 2 : pl.bn;
     pl.tiles_n = (N + out - 1) / out;
     pl.tiles_t = (T + 2 * TILE_M - 1) / (2 * TILE_M);
-    const long tiles = (long)pl.tiles_n * pl.tiles_t;
-    const int pairs = sm_count / 2;
+    const long tiles = (long)pl.tiles_n * pl.tiles_t, waves = (tiles + pairs - 1) / pairs;
     pl.ctas = 2 * (int)(tiles < pairs ? tiles : pairs);
-    const int stage = A_TILE_BYTES + pl.bn / 2 * BLOCK_K;
-    const int stages = (225 * 1024 - OUT_BYTES) / stage;
+    const int stage = A_TILE_BYTES + bn / 2 * BLOCK_K, stages = (225 * 1024 - OUT_BYTES) / stage;
     pl.stages = stages > MAX_STAGES ? MAX_STAGES : stages;
     pl.smem = (size_t)pl.stages * stage + OUT_BYTES + 1024;
-    return pl;
+    const double alone = PAIR_COLUMN_NS * bn > PAIR_BLOCK_NS ? PAIR_COLUMN_NS * bn : PAIR_BLOCK_NS, together = PAIR_BUSY_NS + PAIR_BUSY_COLUMN_NS * bn;
+    const double busy = tiles < pairs ? (double)tiles / pairs : 1.0, block = alone + (together - alone) * busy;
+    const double memory = ((gated ? 2.0 : 1.0) * N * K + (double)T * K) / BYTES_NS, stream = waves * (k_blocks * block + PAIR_TILE_NS);
+    pl.cost = 2500.0 + 10.0 * bn + (stream > memory ? stream : memory);
+}
+
+constexpr int FEW_MOST_TOKENS = 512;       // from here on pairs were the faster ones at every size swept
+
+Plan make_plan(int T, int N, int K, bool gated, int sm_count) {
+    Plan best{}, pl{};
+    best.cost = 1e300;
+    if (T <= FEW_MOST_TOKENS) {
+        const int narrowest = T <= 16 ? 16 : T <= 32 ? 32 : 64, widest = T <= 64 ? narrowest : 128;
+        for (int bn = narrowest; bn <= widest; bn *= 2)
+            for (int splits = MAX_RANKS; splits >= 1; splits--)
+                if (plan_few(pl, T, N, K, gated, sm_count, bn, splits) && pl.cost < best.cost) best = pl;
+    }
+    if (T > 64)
+        for (int bn = PAIR_BN; bn >= 64; bn -= 64) {
+            plan_pairs(pl, T, N, K, gated, sm_count, bn);
+            if (pl.cost < best.cost) best = pl;
+        }
+    return best;
 }
 
 int sm_count_of_current_device() {
@@ -600,11 +730,12 @@ int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const 
                   "gemm_q8_tc: cuTensorMapEncodeTiled refused the operands");
     if (pl.few) {
         const dim3 grid(pl.tiles_n, pl.tiles_t, pl.splits), cluster(1, 1, pl.splits);
+        const int threads = 64 + 32 * few_warps(pl.bn);
         switch (pl.bn) {
-            case 16: return launch_cluster<gemm_q8_few_kernel<16, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
-            case 32: return launch_cluster<gemm_q8_few_kernel<32, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
-            case 64: return launch_cluster<gemm_q8_few_kernel<64, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
-            default: return launch_cluster<gemm_q8_few_kernel<128, EPI, TC>>(grid, FEW_THREADS, cluster, pl.smem, stream, mw, ma, p);
+            case 16: return launch_cluster<gemm_q8_few_kernel<16, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
+            case 32: return launch_cluster<gemm_q8_few_kernel<32, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
+            case 64: return launch_cluster<gemm_q8_few_kernel<64, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
+            default: return launch_cluster<gemm_q8_few_kernel<128, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
         }
     }
     // (TMA writes whole pieces of 16 bytes: where the last of a row is not whole, it would write what lies between the rows)
@@ -614,6 +745,17 @@ int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const 
 }
 
 }  // namespace
+
+// How a product of T tokens, N outputs (gated: of 2N weight rows) and K would be run on a device of sm_count SMs (0: the current one): out[0] the kernel for few
+// tokens, [1] the tile's other side (tokens, or a pair's weight rows), [2] stages of the ring, [3] the cut of K, [4] k blocks of a part, [5] CTAs, [6] bytes of
+// shared memory.  Nothing is launched.
+HYMT2_API int hymt2_gemm_q8_describe(int T, int N, int K, int gated, int sm_count, long* out) {
+    HYMT2_REQUIRE(T > 0 && N > 0 && K > 0 && K <= MAX_K && out, "gemm_q8_describe: bad arguments");
+    const Plan pl = make_plan(T, N, K, gated != 0, sm_count > 0 ? sm_count : sm_count_of_current_device());
+    const long v[7] = {pl.few, pl.bn, pl.stages, pl.splits, pl.k_blocks_per_split, pl.ctas, (long)pl.smem};
+    for (int i = 0; i < 7; i++) out[i] = v[i];
+    return HYMT2_OK;
+}
 
 // C[T, N] (ldc) = epilogue(A[T, K] (lda) · W[N, K]^T (ldw)) with the scales of A's rows and W's; gated: W has 2N rows.  weights_settled: W and its
 // scales were complete before the kernel in front of this one was launched, so they are fetched while that one still runs.

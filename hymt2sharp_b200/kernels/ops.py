@@ -2488,3 +2488,10 @@ def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: tor
         return
     _check(_lib().hymt2_gemm_q8_tc(out.data_ptr(), code, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), T, N, K, lda, ldw, ldo,
                                    epilogue, 1 if weights_settled else 0, status.data_ptr(), _raw_stream(), *rule), "gemm_q8_tc")
+
+
+def gemm_q8_describe(tokens: int, out_features: int, inner: int, gated: bool, sm_count: int = 0) -> dict:
+    """How gemm_q8_tc would run a product (of 2 * out_features weight rows if gated) on a device of sm_count SMs (0: the current one)."""
+    out = (c_long * 7)()
+    _check(_lib().hymt2_gemm_q8_describe(c_int(tokens), c_int(out_features), c_int(inner), c_int(bool(gated)), c_int(sm_count), out), "gemm_q8_describe", 0)
+    return dict(zip(("few", "width", "stages", "splits", "k_blocks", "ctas", "shared_bytes"), out))

@@ -79,3 +79,30 @@ def test_products_that_are_not_taken():
                          (dict(out=torch.empty(1, 2), a=long_a, a_scale=torch.empty(1), w=long_w, w_scale=torch.empty(2)), "do not go together")):
         with pytest.raises(ops.KernelError, match=what):
             ops.gemm_q8_tc(**{**ok, **change})
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_plans_stay_within_the_machine(gated):
+    """Shared memory, tensor memory, clusters and the cover of K, over the range of sizes; nothing is launched."""
+    from hymt2sharp_b200.kernels import build
+    try:
+        build.find_nvcc()
+    except build.BuildError as err:
+        pytest.skip(str(err))
+    sizes = [1, 2, 15, 16, 17, 33, 64, 65, 100, 128, 129, 200, 257, 500, 512, 513, 1000, 4096, 30000]
+    for T in sizes + [200000]:
+        for N in [1, 100, 128, 129, 500, 2048, 6144, 28672, 152064]:
+            for K in [1, 64, 128, 129, 500, 2048, 14336, ops.Q8_MAX_INNER]:
+                for sms in (148, 132):
+                    p = ops.gemm_q8_describe(T, N, K, gated, sms)
+                    blocks, accs = -(-K // 128), 2 if gated else 1
+                    assert 2 <= p["stages"] <= 12 and 1 <= p["splits"] <= 8
+                    assert p["splits"] * p["k_blocks"] >= blocks > (p["splits"] - 1) * p["k_blocks"]
+                    if p["few"]:
+                        assert T <= 512 and p["width"] in (16, 32, 64, 128) and accs * p["width"] <= 256
+                        stage, sums = accs * 16384 + p["width"] * 128, accs * p["width"] * 512
+                        assert p["shared_bytes"] >= max(p["stages"] * stage, sums) + 1024 and p["shared_bytes"] <= 226 * 1024
+                        assert p["ctas"] == -(-N // 128) * -(-T // p["width"]) * p["splits"]
+                    else:
+                        assert T > 64 and p["splits"] == 1 and p["width"] in (64, 128, 192, 256) and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= sms
+                        assert p["stages"] * (16384 + p["width"] * 64) + 32768 + 1024 == p["shared_bytes"] <= 226 * 1024
