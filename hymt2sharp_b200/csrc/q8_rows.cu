@@ -28,32 +28,29 @@ __device__ __forceinline__ RowCode row_code(float top) {
     return c;
 }
 
-// t = x inv is within 127 * 2^-23 = 1.6e-5 of the quotient v = 127 x / top, so the nearest whole number of t is that of v unless t lies within
-// 2e-5 of a border b (a whole number and a half).  There the sign of 127 x - b top decides: 127 x is hi + lo without an error, hi - b top is
+// x inv is within 127 * 2^-24 = 8e-6 of the quotient 127 x / top, so the nearest whole number r of the one is that of the other unless the quotient
+// lies within 2e-5 of a border b (a whole number and a half).  There the sign of 127 x - b top decides: 127 x is hi + lo without an error, hi - b top is
 // a multiple of half of top's last place and small, so both differences are exact.
 constexpr float NEAR_BORDER = 0.49998f;
-__device__ __noinline__ float q8_settle(float x, float r, float e, float top) {
-    const float b = r + copysignf(0.5f, e);
-    const float hi = 127.0f * x, lo = fmaf(127.0f, x, -hi);
-    const float d = fmaf(-b, top, hi) + lo;
-    return d == 0.f ? rintf(b) : d > 0.f ? b + 0.5f : b - 0.5f;
-}
-// x of a row that is all numbers -> the whole number, in the lowest byte.  Adding 1.5 * 2^23 rounds to a whole number (ties to even), whose two's
-// complement then fills the lowest bits.
+// Adding 1.5 * 2^23 rounds to a whole number (ties to even), whose two's complement then fills the lowest bits.
 constexpr float WHOLE = 12582912.0f;
+// entries x (times c.f) of a row that is all numbers -> the whole numbers, in the lowest bytes
 template <int V> __device__ __forceinline__ void q8_of(const float (&x)[V], const RowCode& c, uint32_t (&code)[V]) {
-    bool near = false;
+    float far = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float t = x[i] * c.inv, w = t + WHOLE;
+        const float w = __fmaf_rn(x[i], c.inv, WHOLE);
         code[i] = __float_as_uint(w);
-        near |= fabsf(t - (w - WHOLE)) > NEAR_BORDER;
+        far = fmaxf(far, fabsf(__fmaf_rn(x[i], c.inv, WHOLE - w)));
     }
-    if (near) {
+    if (far > NEAR_BORDER) {      // (one entry in 200 of bfloat16 rows is exactly half way: half of the largest one, say)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const float t = x[i] * c.inv, r = rintf(t);
-            if (fabsf(t - r) > NEAR_BORDER) code[i] = __float_as_uint(q8_settle(x[i], r, t - r, c.top) + WHOLE);
+            const float r = __uint_as_float(code[i]) - WHOLE, e = __fmaf_rn(x[i], c.inv, -r);
+            if (fabsf(e) > NEAR_BORDER) {
+                const float b = r + copysignf(0.5f, e), hi = 127.0f * x[i], d = __fmaf_rn(-b, c.top, hi) + __fmaf_rn(127.0f, x[i], -hi);
+                code[i] = __float_as_uint((d == 0.f ? rintf(b) : d > 0.f ? b + 0.5f : b - 0.5f) + WHOLE);
+            }
         }
     }
 }
@@ -80,29 +77,33 @@ template <bool WARP> struct Place {
     }
 };
 
-// the entries [8 (c threads + tid), + 8) (VEC) or c 8 threads + tid, + threads, ... of a row as float32; zeros behind the row's end
-template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* row, int c, int tid, int threads, int width, float (&v)[8]) {
+// group c of a thread's entries of a row as they are stored; zeros behind the row's end
+template <typename T> struct Eight { Pack<T, 16 / (int)sizeof(T)> p[(int)sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ T& at8(Eight<T>& e, int i) { return e.p[i / (16 / (int)sizeof(T))].v[i % (16 / (int)sizeof(T))]; }
+template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* row, int c, int tid, int threads, int width, Eight<T>& e) {
+    constexpr int N = 16 / (int)sizeof(T);
     if constexpr (VEC) {
         const int at = 8 * (c * threads + tid);
         if (at + 8 <= width) {
-            constexpr int N = 16 / sizeof(T);
 #pragma unroll
-            for (int h = 0; h < 8; h += N) {
-                const Pack<T, N> p = load_pack<T, N>(row + at + h);
-#pragma unroll
-                for (int i = 0; i < N; i++) v[h + i] = to_float(p.v[i]);
-            }
+            for (int h = 0; h < 8 / N; h++) e.p[h] = load_pack<T, N>(row + at + h * N);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = at + i < width ? to_float(row[at + i]) : 0.f;
+            for (int i = 0; i < 8; i++) at8(e, i) = at + i < width ? row[at + i] : from_float<T>(0.f);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int at = (c * 8 + i) * threads + tid;
-            v[i] = at < width ? to_float(row[at]) : 0.f;
+            at8(e, i) = at < width ? row[at] : from_float<T>(0.f);
         }
     }
+}
+template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* row, int c, int tid, int threads, int width, float (&v)[8]) {
+    Eight<T> e;
+    load8<VEC>(row, c, tid, threads, width, e);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = to_float(at8(e, i));
 }
 template <bool VEC, typename T> __device__ __forceinline__ void store8(T* row, int c, int tid, int threads, int width, const float (&v)[8]) {
     if constexpr (VEC) {
@@ -170,25 +171,30 @@ template <bool WARP, bool SUM> __device__ __forceinline__ void over_row(float& m
 }
 
 template <typename TX, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
+__global__ void __launch_bounds__(WARP ? 256 : 1024, WARP ? 1 : 2) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
     __shared__ float2 scratch[32];
     pdl_launch_dependents();
     pdl_wait();
     const Place<WARP> at(rows);
     if (!at.in) return;
     const TX* src = x + at.row * ldx;
-    float v[CH][8], most = 0.f, none = 0.f;
-    // CH loads are in flight before the first is used
+    Eight<TX> x8[CH];             // (as they are stored: half the registers of float32 for bfloat16)
+    float most = 0.f, none = 0.f;
 #pragma unroll
-    for (int c = 0; c < CH; c++) load8<VEC>(src, c, at.tid, at.threads, width, v[c]);
+    for (int c = 0; c < CH; c++) load8<VEC>(src, c, at.tid, at.threads, width, x8[c]);
 #pragma unroll
     for (int c = 0; c < CH; c++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) most = max_abs(most, v[c][i]);
+        for (int i = 0; i < 8; i++) most = max_abs(most, to_float(at8(x8[c], i)));
     over_row<WARP, false>(most, none, scratch);
     const RowCode code = row_code(most);
 #pragma unroll
-    for (int c = 0; c < CH; c++) store_codes<VEC>(q + at.row * ldq, c, at.tid, at.threads, width, v[c], code);
+    for (int c = 0; c < CH; c++) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_float(at8(x8[c], i));
+        store_codes<VEC>(q + at.row * ldq, c, at.tid, at.threads, width, v, code);
+    }
     if (at.tid == 0) scale[at.row] = code.s;
 }
 
@@ -204,7 +210,7 @@ struct NormQ8Params {
 };
 
 template <typename TX, typename TA, typename TG, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_q8_kernel(NormQ8Params p) {
+__global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP && CH == 1 ? 2 : 1) rmsnorm_q8_kernel(NormQ8Params p) {
     __shared__ float2 scratch[32];
     pdl_launch_dependents();
     pdl_wait();
