@@ -11,27 +11,28 @@
 namespace {
 
 struct RowCode {
-    float f, inv, top;    // a power of two that keeps what follows in range; 127 / (max|x| f); max|x| f
-    float s;              // the scale
+    float f, inv, low, top;   // a power of two that keeps what follows in range; about 127 / (max|x| f), and what that leaves of it; max|x| f
     bool none;            // zeros: nothing in the row, or nothing that is a number
 };
 
 // `top`: the largest |x|, infinity and NaN included
 __device__ __forceinline__ RowCode row_code(float top) {
     RowCode c;
-    const bool finite = top < __uint_as_float(0x7f800000u);
-    c.none = !finite || top == 0.f;
+    c.none = !(top < __uint_as_float(0x7f800000u)) || top == 0.f;
     c.f = top > 0x1p100f ? 0x1p-60f : top < 0x1p-60f ? 0x1p90f : 1.0f;
     c.top = top * c.f;
-    c.inv = 127.0f / c.top;
-    c.s = finite ? top / 127.0f : __uint_as_float(0x7fc00000u);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(c.inv) : "f"(c.top));
+    c.low = c.inv;
+    c.inv *= 127.0f;
+    c.low *= __fmaf_rn(-c.inv, c.top, 127.0f);
     return c;
 }
+__device__ __forceinline__ float row_scale(float top) { return top < __uint_as_float(0x7f800000u) ? top / 127.0f : __uint_as_float(0x7fc00000u); }
 
-// x inv is within 127 * 2^-24 = 8e-6 of the quotient 127 x / top, so the nearest whole number r of the one is that of the other unless the quotient
-// lies within 2e-5 of a border b (a whole number and a half).  There the sign of 127 x - b top decides: 127 x is hi + lo without an error, hi - b top is
+// x inv is within 127 (2^-23 + 2^-24) = 2.3e-5 of the quotient 127 x / top (the approximate reciprocal's last place, a rounding), so the nearest whole number r of the one is that of the other unless the quotient
+// lies within 3e-5 of a border b (a whole number and a half).  There the sign of 127 x - b top decides: 127 x is hi + lo without an error, hi - b top is
 // a multiple of half of top's last place and small, so both differences are exact.
-constexpr float NEAR_BORDER = 0.49998f;
+constexpr float NEAR_BORDER = 0.49997f;
 // Adding 1.5 * 2^23 rounds to a whole number (ties to even), whose two's complement then fills the lowest bits.
 constexpr float WHOLE = 12582912.0f;
 // entries x (times c.f) of a row that is all numbers -> the whole numbers, in the lowest bytes
@@ -43,7 +44,7 @@ template <int V> __device__ __forceinline__ void q8_of(const float (&x)[V], cons
         code[i] = __float_as_uint(w);
         far = fmaxf(far, fabsf(__fmaf_rn(x[i], c.inv, WHOLE - w)));
     }
-    if (far > NEAR_BORDER) {      // (one entry in 200 of bfloat16 rows is exactly half way: half of the largest one, say)
+    if (far > NEAR_BORDER) {      // (one float32 in 30,000)
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float r = __uint_as_float(code[i]) - WHOLE, e = __fmaf_rn(x[i], c.inv, -r);
@@ -52,6 +53,16 @@ template <int V> __device__ __forceinline__ void q8_of(const float (&x)[V], cons
                 code[i] = __float_as_uint((d == 0.f ? rintf(b) : d > 0.f ? b + 0.5f : b - 0.5f) + WHOLE);
             }
         }
+    }
+}
+// The same for bfloat16 entries, without a special case: 127 x / top is x (inv + low) within 4e-12, summed so that t is that rounded once.  A border is a
+// float32, so a quotient on one stays there (then ties go to even), and one of bfloat16 numbers that is not on a border is 2^-17 away from it at least
+// (1 / (2 * 255 * 2^8)), twice what the rounding of t moves.
+template <int V> __device__ __forceinline__ void q8_of_short(const float (&x)[V], const RowCode& c, uint32_t (&code)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float p = __fmul_rn(x[i], c.inv), t = __fadd_rn(p, __fmaf_rn(x[i], c.low, __fmaf_rn(x[i], c.inv, -p)));
+        code[i] = __float_as_uint(__fadd_rn(t, WHOLE));
     }
 }
 __device__ __forceinline__ uint32_t pack4(const uint32_t* c) { return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410); }
@@ -78,7 +89,7 @@ template <bool WARP> struct Place {
 };
 
 // group c of a thread's entries of a row as they are stored; zeros behind the row's end
-template <typename T> struct Eight { Pack<T, 16 / (int)sizeof(T)> p[(int)sizeof(T) / 2]; };
+template <typename T> struct alignas(16) Eight { Pack<T, 16 / (int)sizeof(T)> p[(int)sizeof(T) / 2]; };
 template <typename T> __device__ __forceinline__ T& at8(Eight<T>& e, int i) { return e.p[i / (16 / (int)sizeof(T))].v[i % (16 / (int)sizeof(T))]; }
 template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* row, int c, int tid, int threads, int width, Eight<T>& e) {
     constexpr int N = 16 / (int)sizeof(T);
@@ -99,11 +110,37 @@ template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* r
         }
     }
 }
+// the group as float32, and the largest of `most` and its sizes (a bfloat16's bits are the upper half of the float32's; sizes are compared two at a time)
+template <typename T> __device__ __forceinline__ void floats8(const Eight<T>& e, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_float(e.p[i / 4].v[i % 4]);
+    }
+}
+template <typename T> __device__ __forceinline__ float most8(const Eight<T>& e, float most) {
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
+        uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        return __uint_as_float(max(__float_as_uint(most), max(m << 16, m & 0xffff0000u)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) most = max_abs(most, e.p[i / 4].v[i % 4]);
+        return most;
+    }
+}
 template <bool VEC, typename T> __device__ __forceinline__ void load8(const T* row, int c, int tid, int threads, int width, float (&v)[8]) {
     Eight<T> e;
     load8<VEC>(row, c, tid, threads, width, e);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = to_float(at8(e, i));
+    floats8(e, v);
 }
 template <bool VEC, typename T> __device__ __forceinline__ void store8(T* row, int c, int tid, int threads, int width, const float (&v)[8]) {
     if constexpr (VEC) {
@@ -129,7 +166,7 @@ template <bool VEC, typename T> __device__ __forceinline__ void store8(T* row, i
         }
     }
 }
-template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* row, int c, int tid, int threads, int width, float (&v)[8], const RowCode& code) {
+template <bool VEC, bool SHORT> __device__ __forceinline__ void store_codes(int8_t* row, int c, int tid, int threads, int width, float (&v)[8], const RowCode& code) {
     uint32_t w[8];
     if (code.none) {
 #pragma unroll
@@ -139,7 +176,8 @@ template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* row, int
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] *= code.f;
         }
-        q8_of(v, code, w);
+        if constexpr (SHORT) q8_of_short(v, code, w);
+        else q8_of(v, code, w);
     }
     if constexpr (VEC) {
         const int at = 8 * (c * threads + tid);
@@ -171,7 +209,7 @@ template <bool WARP, bool SUM> __device__ __forceinline__ void over_row(float& m
 }
 
 template <typename TX, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 256 : 1024, WARP ? 1 : 2) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
+__global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, WARP ? 1 : CH == 4 && sizeof(TX) == 2 ? 3 : VEC ? 2 : 1) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
     __shared__ float2 scratch[32];
     pdl_launch_dependents();
     pdl_wait();
@@ -183,19 +221,16 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, WARP ? 1 : 2) quantize_q8_k
 #pragma unroll
     for (int c = 0; c < CH; c++) load8<VEC>(src, c, at.tid, at.threads, width, x8[c]);
 #pragma unroll
-    for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) most = max_abs(most, to_float(at8(x8[c], i)));
+    for (int c = 0; c < CH; c++) most = most8(x8[c], most);
     over_row<WARP, false>(most, none, scratch);
     const RowCode code = row_code(most);
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = to_float(at8(x8[c], i));
-        store_codes<VEC>(q + at.row * ldq, c, at.tid, at.threads, width, v, code);
+        floats8(x8[c], v);
+        store_codes<VEC, sizeof(TX) == 2>(q + at.row * ldq, c, at.tid, at.threads, width, v, code);
     }
-    if (at.tid == 0) scale[at.row] = code.s;
+    if (at.tid == 0) scale[at.row] = row_scale(most);
 }
 
 struct NormQ8Params {
@@ -210,7 +245,7 @@ struct NormQ8Params {
 };
 
 template <typename TX, typename TA, typename TG, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP && CH == 1 ? 2 : 1) rmsnorm_q8_kernel(NormQ8Params p) {
+__global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP && CH == 1 && VEC ? 2 : 1) rmsnorm_q8_kernel(NormQ8Params p) {
     __shared__ float2 scratch[32];
     pdl_launch_dependents();
     pdl_wait();
@@ -243,8 +278,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP && CH == 1 ? 2 : 1) r
     over_row<WARP, true>(most, ss, scratch);
     const RowCode code = row_code(most);
 #pragma unroll
-    for (int c = 0; c < CH; c++) store_codes<VEC>(p.q + at.row * p.ldq, c, at.tid, at.threads, p.width, v[c], code);
-    if (at.tid == 0) p.scale[at.row] = code.s * (1.0f / sqrtf(ss / (float)p.width + p.eps));
+    for (int c = 0; c < CH; c++) store_codes<VEC, false>(p.q + at.row * p.ldq, c, at.tid, at.threads, p.width, v[c], code);
+    if (at.tid == 0) p.scale[at.row] = row_scale(most) * (1.0f / sqrtf(ss / (float)p.width + p.eps));
 }
 
 // Rows that the registers of 1,024 threads do not hold are read twice, the second time out of L2.
@@ -268,9 +303,9 @@ __global__ void __launch_bounds__(1024) quantize_q8_long_kernel(int8_t* q, long 
     for (int c = 0; c * 8192 < width; c++) {
         float v[8];
         load8<VEC>(src, c, threadIdx.x, 1024, width, v);
-        store_codes<VEC>(q + (size_t)blockIdx.x * ldq, c, threadIdx.x, 1024, width, v, code);
+        store_codes<VEC, sizeof(TX) == 2>(q + (size_t)blockIdx.x * ldq, c, threadIdx.x, 1024, width, v, code);
     }
-    if (threadIdx.x == 0) scale[blockIdx.x] = code.s;
+    if (threadIdx.x == 0) scale[blockIdx.x] = row_scale(most);
 }
 
 template <typename TX, typename TA, typename TG, bool VEC>
@@ -309,9 +344,9 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(NormQ8Params p) {
         load8<VEC>((const TG*)p.gain, c, threadIdx.x, 1024, p.width, g);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] *= g[i];
-        store_codes<VEC>(p.q + r * p.ldq, c, threadIdx.x, 1024, p.width, v, code);
+        store_codes<VEC, false>(p.q + r * p.ldq, c, threadIdx.x, 1024, p.width, v, code);
     }
-    if (threadIdx.x == 0) p.scale[r] = code.s * (1.0f / sqrtf(ss / (float)p.width + p.eps));
+    if (threadIdx.x == 0) p.scale[r] = row_scale(most) * (1.0f / sqrtf(ss / (float)p.width + p.eps));
 }
 
 // A warp takes pieces of 4 x 32 groups of 16 output bytes of a row (VEC), or 512 single entries.
@@ -357,11 +392,12 @@ inline bool whole(const void* p, long ld, int size) { return (uintptr_t)p % 16 =
 
 // How a row is shared: groups of 8 entries a thread, a warp or a block a row, threads of a block.
 struct Share { int ch, threads, blocks; bool warp; };
-Share share_of(int rows, int width, bool norm) {
+constexpr int FEW_ROWS = 296;
+Share share_of(int rows, int width, bool norm, bool vec) {
     const int groups = (width + 7) / 8;
     if (groups <= 128) return Share{groups <= 32 ? 1 : groups <= 64 ? 2 : 4, 256, (rows + 7) / 8, true};
     // (a norm's sums are added in an order that the share decides, so its share hangs on the width alone)
-    const int ch = norm && groups <= 1024 ? 1 : 2;
+    const int ch = !norm && vec && rows > FEW_ROWS ? 4 : groups <= 1024 ? 1 : 2;
     return Share{ch, ((groups + ch - 1) / ch + 31) / 32 * 32, rows, false};
 }
 
@@ -369,7 +405,7 @@ template <typename TX, bool VEC>
 int run_quantize(const Share& s, int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width, cudaStream_t stream) {
 #define HYMT2_RUN(CH, WARP) launch_pdl(quantize_q8_kernel<TX, CH, WARP, VEC>, dim3(s.blocks), dim3(s.threads), 0, stream, q, ldq, scale, x, ldx, rows, width)
     if (s.warp) s.ch == 1 ? HYMT2_RUN(1, true) : s.ch == 2 ? HYMT2_RUN(2, true) : HYMT2_RUN(4, true);
-    else HYMT2_RUN(2, false);
+    else s.ch == 1 ? HYMT2_RUN(1, false) : s.ch == 2 ? HYMT2_RUN(2, false) : HYMT2_RUN(4, false);
 #undef HYMT2_RUN
     return hymt2_check_launch("quantize_q8");
 }
@@ -394,8 +430,9 @@ HYMT2_API int hymt2_quantize_q8(void* q, long ldq, float* scale, const void* x, 
                        (int8_t*)q, ldq, scale, (const TX*)x, ldx, width);
             return hymt2_check_launch("quantize_q8");
         }
-        const Share s = share_of(rows, width, false);
-        if (whole(x, ldx, sizeof(TX))) return run_quantize<TX, true>(s, (int8_t*)q, ldq, scale, (const TX*)x, ldx, rows, width, stream);
+        const bool vec = whole(x, ldx, sizeof(TX));
+        const Share s = share_of(rows, width, false, vec);
+        if (vec) return run_quantize<TX, true>(s, (int8_t*)q, ldq, scale, (const TX*)x, ldx, rows, width, stream);
         return run_quantize<TX, false>(s, (int8_t*)q, ldq, scale, (const TX*)x, ldx, rows, width, stream);
     });
 }
@@ -424,7 +461,7 @@ HYMT2_API int hymt2_rmsnorm_q8(void* q, long ldq, float* scale, const void* x, i
     HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "rmsnorm_q8: rows of integers must start on 16 bytes");
     HYMT2_REQUIRE(!total || add, "rmsnorm_q8: the sums have a place, but nothing is added");
     const NormQ8Params p{(int8_t*)q, scale, x, add, total, gain, ldq, ldx, ldadd, ldt, rows, width, eps};
-    const Share s = share_of(rows, width, true);
+    const Share s = share_of(rows, width, true, true);
     HYMT2_DISPATCH_DTYPE(x_dtype, TX, HYMT2_DISPATCH_DTYPE(add_dtype, TA, HYMT2_DISPATCH_DTYPE(gain_dtype, TG, {
         const bool vec = whole(x, ldx, sizeof(TX)) && (!add || whole(add, ldadd, sizeof(TA))) && (!total || whole(total, ldt, sizeof(TX))) &&
                          (uintptr_t)gain % 16 == 0;
