@@ -13,7 +13,7 @@ so prompts are token ids ("12,7,99" or "12 7 99") and replies are printed as ids
   --backend NAME     auto or cuda (cpu, metal and vulkan do not exist here)
   --profile          per-kernel times of the prefill and of the decode steps (the Benchmark program's switch,
                      src/HyMT2Sharp.Benchmark/Program.cs:243-261); kernels then run one after the other
-and beyond the reference: --dtype, --temperature, --top-k, --top-p, --min-p,
+and beyond the reference: --dtype, --weights (int8: the layers' matrices as 8-bit integers), --temperature, --top-k, --top-p, --min-p,
 --repeat-penalty, --penalty-window, --seed, --stop-ids, --max-context, --max-batch,
 --random CONFIG.json --weights-seed N --sigma S (write random weights into --model first).
 """
@@ -44,6 +44,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--threads", type=int, default=0)
     ap.add_argument("--backend", default="auto")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "int8"], help="int8: the layers' matrices are kept as 8-bit integers")
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
@@ -81,7 +82,8 @@ def main(argv=None) -> int:
     print(f"HyMT2Sharp-B200  model={args.model}")
     print(f"threads={'auto' if args.threads <= 0 else args.threads} (unused)  backend=cuda  dtype={args.dtype}")
     t0 = time.perf_counter()
-    engine = Engine(args.model, dtype=args.dtype, max_tokens=args.max_context, max_batch=args.max_batch)
+    engine = Engine(args.model, dtype=args.dtype, max_tokens=args.max_context, max_batch=args.max_batch,
+                    weights=None if args.weights == "stored" else args.weights)
     c = engine.config
     if hasattr(c, "num_attention_heads"):
         mixers = f"heads={c.num_attention_heads}/{c.num_key_value_heads}"

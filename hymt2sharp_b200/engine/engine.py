@@ -18,8 +18,10 @@ from ..cache import PagedCache
 from ..config.registry import load_config
 from ..kernels import build as kernel_build, ops
 from ..parts.base import StepContext
+from ..parts.linear8 import WEIGHT_KINDS
 from ..weights.loader import load_checkpoint
 from .model import DecoderModel
+from .spec import with_weights
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32,
           torch.bfloat16: torch.bfloat16, torch.float32: torch.float32}
@@ -105,18 +107,26 @@ def make_context(cache, entries: list, vocab: int, dtype, device, status, meta_b
 class Engine:
     def __init__(self, model_dir: str, dtype="bfloat16", max_tokens: int = 8192, max_batch: int = 8,
                  block_tokens: int = 64, device="cuda:0", max_sequence_tokens: int | None = None,
-                 spec_override=None):
+                 spec_override=None, weights: str | None = None):
+        """`weights` "int8": the layers' matrices are kept as 8-bit integers with a scale for each output channel and multiplied with rows of
+        8-bit integers (spec.with_weights says for which architectures); None: as the checkpoint stores them."""
         if dtype not in DTYPES:
             raise EngineError(f"dtype must be 'bfloat16' or 'float32', got {dtype!r}")
+        if weights not in WEIGHT_KINDS:
+            raise EngineError(f"weights must be one of {', '.join(repr(k) for k in WEIGHT_KINDS)}, got {weights!r}")
         self.dtype = DTYPES[dtype]
         self.device = require_gpu(device)
         kernel_build.load_library()  # fails loudly when the CUDA library cannot be built or loaded
         self.architecture, self.config = load_config(model_dir)
         spec = self.architecture.build_spec(self.config) if spec_override is None else spec_override(self.config)
+        try:
+            spec = with_weights(spec, weights)
+        except ValueError as err:
+            raise EngineError(str(err)) from None
         self.model = DecoderModel(spec)
-        weights = load_checkpoint(model_dir, self.model.tensors(), spec.ignorable_tensors)
+        stored = load_checkpoint(model_dir, self.model.tensors(), spec.ignorable_tensors)
         with torch.cuda.device(self.device):
-            self.model.load(weights, self.device, self.dtype)
+            self.model.load(stored, self.device, self.dtype)
             self.cache = PagedCache(self.model.groups, self.dtype, self.device, capacity_tokens=max_tokens,
                                     block_tokens=block_tokens, max_slots=max_batch,
                                     state_bytes=self.model.state_bytes, max_sequence_tokens=max_sequence_tokens)

@@ -116,8 +116,9 @@ class DecoderModel:
         if dtype == torch.bfloat16:
             # a tensor stored in 32-bit stays so; for a MATRIX that means its product runs on the CUDA-core kernel,
             # many times slower than the tensor cores.  That is a property of the checkpoint worth saying aloud.
+            narrowed = {name for b in self.blocks for name in b.tensors()} if s.weights is not None else set()     # (they became integers)
             wide = [name for name, spec in self.tensors().items()
-                    if len(spec.shape) == 2 and name in weights and weights[name].dtype == torch.float32]
+                    if len(spec.shape) == 2 and name in weights and weights[name].dtype == torch.float32 and name not in narrowed]
             if wide:
                 import warnings
                 warnings.warn(f"{len(wide)} matrices of the checkpoint are stored in 32-bit (first: {wide[0]}); the bfloat16 "
@@ -134,7 +135,7 @@ class DecoderModel:
         def visit(obj, depth=0):
             nonlocal total
             if isinstance(obj, torch.Tensor):
-                if obj.is_floating_point() and obj.data_ptr() not in seen:
+                if (obj.is_floating_point() or obj.dtype == torch.int8) and obj.data_ptr() not in seen:
                     seen.add(obj.data_ptr())
                     total += obj.numel() * obj.element_size()
             elif isinstance(obj, (list, tuple)):

@@ -4,9 +4,10 @@ norm and the output head come from.  An architecture's builder turns its
 configuration into this; nothing below it knows the architecture."""
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 from ..parts.base import PartSpec
+from ..parts.linear8 import check_weights
 
 
 @dataclass
@@ -56,6 +57,7 @@ class ModelSpec:
     residual_streams: int | None = None
     bigram: Bigram | None = None      # (None: the embedding's rows alone)
     join: str | None = None           # checkpoint name of the [hidden, 2 hidden] matrix of the runs that say `joins`
+    weights: str | None = None        # "int8": the layers' matrices are kept as 8-bit integers (with_weights)
     positions: str | None = None      # checkpoint name of a [max_positions, hidden] table: row p is added at position p (not scaled)
 
     def __post_init__(self):
@@ -77,3 +79,26 @@ class ModelSpec:
                     raise ValueError(f"order[{i}] reads the cache of entry {run.cache_from}, which does not run before it")
                 if self.order[run.cache_from].cache_from is not None:
                     raise ValueError(f"order[{i}] reads the cache of entry {run.cache_from}, which has none of its own")
+
+
+# the parts whose matrices can be kept as 8-bit integers (parts.linear8)
+INT8_MIXERS, INT8_FEED_FORWARDS = ("gqa_attention",), ("swiglu", "clamped_glu")
+
+
+def with_weights(spec: ModelSpec, weights: str | None) -> ModelSpec:
+    """The same model with its layers' matrices kept as `weights` says: None, as they are stored; "int8", as 8-bit integers with a scale for each output
+    channel, multiplied with rows of 8-bit integers that have a scale for each token.  Embedding and output head stay as they are.  Layers of other
+    kinds than a pre-norm block of grouped-query attention and a gated feed-forward are refused."""
+    check_weights(weights)
+    if weights is None:
+        return spec
+    layers = []
+    for i, layer in enumerate(spec.layers):
+        p = layer.params
+        if layer.kind != "pre_norm" or p["mixer"].kind not in INT8_MIXERS or p["feed_forward"].kind not in INT8_FEED_FORWARDS:
+            held = f"{layer.kind}" if layer.kind != "pre_norm" else f"pre_norm of {p['mixer'].kind} and {p['feed_forward'].kind}"
+            raise ValueError(f"weights '{weights}' are built for pre_norm blocks of {', '.join(INT8_MIXERS)} and {' or '.join(INT8_FEED_FORWARDS)}; "
+                             f"layer {i} is {held}")
+        inner = {name: PartSpec(p[name].kind, {**p[name].params, "weights": weights}) for name in ("mixer", "feed_forward")}
+        layers.append(PartSpec(layer.kind, {**p, **inner}))
+    return replace(spec, layers=layers, weights=weights)

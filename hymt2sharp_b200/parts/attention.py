@@ -14,7 +14,8 @@ Beyond that form, chosen by parameters: values of another width than keys (`valu
 own (`own_kv` False), which reads the cache plane of the run that the model's order names for it, with its own queries;
 biases of the q, k and v projections (`q_bias`, `k_bias`, `v_bias`: stored vectors, added before the rotation); and a gate
 per head (`head_gate`: a stored matrix [heads, hidden]; head h's output is multiplied by sigmoid((W_gate x)_h) in front of
-the output projection).
+the output projection).  `weights` "int8" keeps the projections' matrices as 8-bit integers with a scale a row (parts.linear8): x may then be
+8-bit rows, and rotation and cache append run behind the projection.
 The classic form (none of these) runs the fused and tensor-core kernels; the others run the general kernels, and the
 tensor-core attention where it takes the shape.
 """
@@ -28,14 +29,15 @@ from ..cache.allocator import GroupSpec
 from ..kernels import ops
 from ..weights.loader import TensorSpec
 from .base import MixerSlot, PartSpec, Prenormed, RotaryEpilogue, build_part, register_part
-from .linear import Linear, compute_form
+from .linear import compute_form
+from .linear8 import check_weights, make_linear, same_weight
 
 SPLIT_KEYS = 256  # decode: keys per partial, a constant so that the cut depends on nothing else
 
 
 class GQAAttention:
     graph_safe = True  # its forward only launches kernels on the current stream
-    takes_prenormed = True  # x may be a parts.base.Prenormed: the projection applies the norm's row scale itself
+    # takes_prenormed: x may be a parts.base.Prenormed: the projection applies the norm's row scale itself
     can_store = True   # forward(..., store=True) overwrites `residual` with its output instead of adding to it
 
     def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, eps: float, qk_norm,
@@ -43,7 +45,11 @@ class GQAAttention:
                  q_norm: str | None = None, k_norm: str | None = None, window: int | None = None,
                  value_dim: int | None = None, scale: float | None = None, norm_first: bool = False, sink: bool = False,
                  own_kv: bool = True, q_bias: str | None = None, k_bias: str | None = None, v_bias: str | None = None,
-                 head_gate: str | None = None):
+                 head_gate: str | None = None, weights: str | None = None):
+        check_weights(weights)
+        self.weights = weights
+        # a product with 8-bit weights takes 8-bit rows, not a norm's output in two pieces
+        self.takes_prenormed, self.takes_rows8 = weights is None, weights is not None
         if heads % kv_heads:
             raise ValueError(f"{heads} heads are not a multiple of {kv_heads} kv heads")
         if qk_norm not in (False, True, None, "head", "all"):
@@ -105,14 +111,14 @@ class GQAAttention:
     def load(self, weights, device, dtype):
         n = self.names
         rows = [weights[n["q"]]] + ([weights[n["k"]], weights[n["v"]]] if self.own_kv else [])
-        self.qkv = Linear(compute_form(torch.cat(rows, dim=0), device, dtype), role="qkv" if self.own_kv else "q_proj")
-        self.out = Linear(compute_form(weights[n["o"]], device, dtype), ops.EPILOGUE_ACCUMULATE, role="o_proj")
-        self.out_store = Linear(self.out.weight, ops.EPILOGUE_STORE, role="o_proj")
+        self.qkv = make_linear(self.weights, torch.cat(rows, dim=0), device, dtype, role="qkv" if self.own_kv else "q_proj")
+        self.out = make_linear(self.weights, weights[n["o"]], device, dtype, ops.EPILOGUE_ACCUMULATE, role="o_proj")
+        self.out_store = same_weight(self.out, ops.EPILOGUE_STORE)
         if n["qb"] is not None:
             self.bias = torch.cat([weights[name].to(device).float().reshape(-1)
                                    for name in ([n["qb"]] + ([n["kb"], n["vb"]] if self.own_kv else []))]).contiguous()
         if n["g"] is not None:
-            self.gate = Linear(compute_form(weights[n["g"]], device, dtype), role="head_gate")
+            self.gate = make_linear(self.weights, weights[n["g"]], device, dtype, role="head_gate")
         if self.qk_norm:
             self.q_gain = compute_form(weights[n["qn"]], device, dtype)
             self.k_gain = compute_form(weights[n["kn"]], device, dtype) if self.own_kv else None
@@ -137,7 +143,7 @@ class GQAAttention:
         planes = (k_plane, v_plane) if slot.writes else (None, None)
         q = None
         pre = x if isinstance(x, Prenormed) else None
-        if epilogue is not None and x.shape[0] == T:
+        if epilogue is not None and x.shape[0] == T and self.weights is None:
             # projection, rotation, norm and cache append as one kernel, where the kernels have one for the shape
             q = fast.try_project_rope_kv(pre.normed if pre else x, self.qkv.weight, epilogue, ctx, planes, k_plane.dtype,
                                          block_table, self.q_gain, self.k_gain, self.eps, nh, nkv, d,

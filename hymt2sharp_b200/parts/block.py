@@ -3,9 +3,16 @@
 float32; the normed activations have the engine's compute type."""
 from __future__ import annotations
 
+import torch
+
 from ..kernels import ops
 from . import dense
 from .base import PartSpec, Prenormed, build_part, register_part
+
+
+def makes_rows8(norm, part) -> bool:
+    """Whether `norm` can hand `part` 8-bit rows, which a part with 8-bit weights takes."""
+    return getattr(part, "takes_rows8", False) and getattr(norm, "foldable", False) and hasattr(norm, "rows8")
 
 
 class PreNormBlock:
@@ -46,7 +53,10 @@ class PreNormBlock:
         return self.norm1 if getattr(self.mixer, "takes_prenormed", False) else None
 
     def forward(self, residual, ctx, slots) -> None:
-        x = self.norm1.forward(residual, ctx, ctx.dtype)      # what the block before left behind, or the norm's own kernel
+        if makes_rows8(self.norm1, self.mixer):
+            x = self.norm1.rows8(residual, ctx)
+        else:
+            x = self.norm1.forward(residual, ctx, ctx.dtype)      # what the block before left behind, or the norm's own kernel
         if isinstance(x, Prenormed) and not getattr(self.mixer, "takes_prenormed", False):
             x = x.materialize(ctx)
         if self.dense and dense.try_block(self, x, residual, ctx, slots[0]):
@@ -55,9 +65,17 @@ class PreNormBlock:
         ctx.weights_ahead = getattr(self.feed_forward, "first_weights", lambda: None)()
         # the norm that comes next, for a mixer whose last product can prepare it
         ctx.norm_ahead = self.norm2 if getattr(self.feed_forward, "takes_prenormed", False) else None
-        self.mixer.forward(x, residual, ctx, slots[0])
-        ctx.weights_ahead = ctx.norm_ahead = None
-        x = self.norm2.forward(residual, ctx, ctx.dtype)
+        if makes_rows8(self.norm2, self.feed_forward) and getattr(self.mixer, "can_store", False):
+            # the mixer's output waits in the compute type, and the norm's kernel adds it to the residual: one way less over the float32 rows
+            # than a product that adds into them (the rounding of what is added is that of any activation)
+            added = torch.empty(residual.shape, dtype=ctx.dtype, device=residual.device)
+            self.mixer.forward(x, added, ctx, slots[0], store=True)
+            ctx.weights_ahead = ctx.norm_ahead = None
+            x = self.norm2.rows8(residual, ctx, add=added)
+        else:
+            self.mixer.forward(x, residual, ctx, slots[0])
+            ctx.weights_ahead = ctx.norm_ahead = None
+            x = self.norm2.rows8(residual, ctx) if makes_rows8(self.norm2, self.feed_forward) else self.norm2.forward(residual, ctx, ctx.dtype)
         if isinstance(x, Prenormed) and not getattr(self.feed_forward, "takes_prenormed", False):
             x = x.materialize(ctx)
         ctx.norm_ahead = ctx.next_first_norm

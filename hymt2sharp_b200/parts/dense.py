@@ -27,7 +27,7 @@ def takes(block) -> bool:
     from .swiglu import SwiGLU
     mixer, ff = block.mixer, block.feed_forward
     return type(mixer) is GQAAttention and mixer.classic and mixer.head_dim == HEAD and mixer.qk_norm in (None, "head") and type(ff) is SwiGLU \
-        and ff.activation == "silu"
+        and ff.activation == "silu" and mixer.weights is None and ff.weights is None
 
 
 def try_block(block, x, residual: torch.Tensor, ctx, slot) -> bool:

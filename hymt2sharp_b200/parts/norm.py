@@ -12,6 +12,7 @@ from ..kernels import ops
 from ..weights.loader import TensorSpec
 from .base import register_part
 from .linear import compute_form
+from .linear8 import Rows8
 
 
 class RMSNorm:
@@ -52,6 +53,13 @@ class RMSNorm:
         else:
             ops.rmsnorm_groups(out, x, self.gain, self.eps, self.groups, rows_index, scale)
         return out
+
+    def rows8(self, x: torch.Tensor, ctx, add: torch.Tensor | None = None) -> Rows8:
+        """The normed rows as 8-bit integers with a scale each; with `add` the rows x take that addition first, in place.  (A norm in one part.)"""
+        ctx.prenormed = None
+        rows = Rows8.room(x.shape[0], self.dim, x.device)
+        ops.rmsnorm_q8(rows.q, rows.scale, x, self.gain, self.eps, add=add, total=None if add is None else x)
+        return rows
 
     def add_into(self, x: torch.Tensor, residual: torch.Tensor) -> None:
         """residual (float32) += norm(x): a sublayer's output that is normed before it joins the residual stream."""

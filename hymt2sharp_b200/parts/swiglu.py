@@ -7,7 +7,9 @@ The projections may have biases: the gate's and the up projection's are added in
 (or, asked with `bias_later`, by the block, which adds the sublayer's output up anyway: `output_bias`).
 
 `activation` "gelu_tanh" puts the tanh form of GELU in SiLU's place: residual += (gelu_tanh(x·Wg^T) * (x·Wu^T)) · Wd^T.
-The product's epilogue knows SiLU only, so that form stores gate and up side by side and a small kernel follows."""
+The product's epilogue knows SiLU only, so that form stores gate and up side by side and a small kernel follows.
+
+`weights` "int8" keeps the matrices as 8-bit integers with a scale a row (parts.linear8); x may then be 8-bit rows."""
 from __future__ import annotations
 
 import torch
@@ -15,7 +17,7 @@ import torch
 from ..kernels import ops
 from ..weights.loader import TensorSpec
 from .base import register_part
-from .linear import Linear, compute_form
+from .linear8 import check_weights, make_linear, same_weight
 
 
 ACTIVATIONS = {"silu": ops.GATED_SILU, "gelu_tanh": ops.GATED_GELU_TANH}
@@ -40,11 +42,14 @@ def _gated_biases(weights, n: dict, device) -> tuple:
 
 class SwiGLU:
     graph_safe = True  # its forward only launches kernels on the current stream
-    takes_prenormed = True  # x may be a parts.base.Prenormed: the gate/up product applies the norm's row scale itself
+    # takes_prenormed: x may be a parts.base.Prenormed: the gate/up product applies the norm's row scale itself
     can_store = True   # forward(..., store=True) overwrites `residual` with its output instead of adding to it
 
     def __init__(self, hidden: int, intermediate: int, gate_proj: str, up_proj: str, down_proj: str, activation: str = "silu",
-                 gate_bias: str | None = None, up_bias: str | None = None, down_bias: str | None = None):
+                 gate_bias: str | None = None, up_bias: str | None = None, down_bias: str | None = None, weights: str | None = None):
+        check_weights(weights)
+        self.weights = weights
+        self.takes_prenormed, self.takes_rows8 = weights is None, weights is not None
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation '{activation}' is not known (known: {', '.join(ACTIVATIONS)})")
         if (gate_bias is None) != (up_bias is None):
@@ -63,10 +68,10 @@ class SwiGLU:
         stacked = torch.cat([weights[n["g"]], weights[n["u"]]], dim=0)
         fused = self.activation == "silu"
         bias_in, self.output_bias = _gated_biases(weights, n, device)
-        self.gate_up = Linear(compute_form(stacked, device, dtype), ops.EPILOGUE_SWIGLU if fused else ops.EPILOGUE_STORE, role="gate_up",
-                              glu_bias=bias_in)
-        self.down = Linear(compute_form(weights[n["d"]], device, dtype), ops.EPILOGUE_ACCUMULATE, role="down")
-        self.down_store = Linear(self.down.weight, ops.EPILOGUE_STORE, role="down")
+        self.gate_up = make_linear(self.weights, stacked, device, dtype, ops.EPILOGUE_SWIGLU if fused else ops.EPILOGUE_STORE, role="gate_up",
+                                   glu_bias=bias_in)
+        self.down = make_linear(self.weights, weights[n["d"]], device, dtype, ops.EPILOGUE_ACCUMULATE, role="down")
+        self.down_store = same_weight(self.down, ops.EPILOGUE_STORE)
 
     def first_weights(self):
         """The weights that this part's first kernel streams."""
@@ -100,7 +105,10 @@ class ClampedGLU:
     can_store = True
 
     def __init__(self, hidden: int, intermediate: int, limit: float, alpha: float, gate_proj: str, up_proj: str, down_proj: str,
-                 gate_bias: str | None = None, up_bias: str | None = None, down_bias: str | None = None):
+                 gate_bias: str | None = None, up_bias: str | None = None, down_bias: str | None = None, weights: str | None = None):
+        check_weights(weights)
+        self.weights = weights
+        self.takes_rows8 = weights is not None
         if (gate_bias is None) != (up_bias is None):
             raise ValueError("the gate's and the up projection's biases come together or not at all")
         if not limit > 0:
@@ -115,10 +123,10 @@ class ClampedGLU:
     def load(self, weights, device, dtype):
         n = self.names
         bias_in, self.output_bias = _gated_biases(weights, n, device)
-        self.gate_up = Linear(compute_form(torch.cat([weights[n["g"]], weights[n["u"]]], dim=0), device, dtype), ops.EPILOGUE_SWIGLU,
-                              role="gate_up", glu=ops.GluRule("clamped", self.limit, self.alpha), glu_bias=bias_in)
-        self.down = Linear(compute_form(weights[n["d"]], device, dtype), ops.EPILOGUE_ACCUMULATE, role="down")
-        self.down_store = Linear(self.down.weight, ops.EPILOGUE_STORE, role="down")
+        self.gate_up = make_linear(self.weights, torch.cat([weights[n["g"]], weights[n["u"]]], dim=0), device, dtype, ops.EPILOGUE_SWIGLU,
+                                   role="gate_up", glu=ops.GluRule("clamped", self.limit, self.alpha), glu_bias=bias_in)
+        self.down = make_linear(self.weights, weights[n["d"]], device, dtype, ops.EPILOGUE_ACCUMULATE, role="down")
+        self.down_store = same_weight(self.down, ops.EPILOGUE_STORE)
 
     def first_weights(self):
         return self.gate_up.weight if self.gate_up is not None else None
