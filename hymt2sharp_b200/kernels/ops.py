@@ -2373,36 +2373,44 @@ Q8_MAX_INNER = 131071     # entries of a row that a product takes: 128 * 128 of 
 def q8_rows(rows: int, width: int, device) -> torch.Tensor:
     """Room for [rows, width] 8-bit integers in the layout of the 8-bit kernels: every row starts on 16 bytes.  (What lies between two
     rows belongs to neither.)"""
-    return torch.empty((rows, -(-width // 16) * 16), dtype=torch.int8, device=device)[:, :width]
+    return torch.empty_strided((rows, width), ((width + 15) & ~15, 1), dtype=torch.int8, device=device)
 
 
-def _q8(t: torch.Tensor, scale: torch.Tensor, name: str) -> int:
-    """Checks a matrix of 8-bit rows and its scales; the rows' distance."""
-    if t.dtype != torch.int8 or t.dim() != 2:
-        raise KernelError(f"{name} must be an int8 matrix, got {t.dtype} {tuple(t.shape)}")
-    rows, width = t.shape
-    ld = t.stride(0) if rows > 1 else -(-width // 16) * 16
-    if (t.stride(1) != 1 and width > 1) or ld % 16 or ld < width or t.data_ptr() % 16:
+# (These checks stand in front of kernels of a few microseconds, so they ask a tensor for each thing once.)
+def _q8(t: torch.Tensor, scale: torch.Tensor, name: str) -> tuple:
+    """Checks a matrix of 8-bit rows and its scales: (rows, width, the rows' distance)."""
+    shape = t.shape
+    if t.dtype is not torch.int8 or len(shape) != 2:
+        raise KernelError(f"{name} must be an int8 matrix, got {t.dtype} {tuple(shape)}")
+    rows, width = shape
+    ld, step = t.stride()
+    if rows < 2:
+        ld = (width + 15) & ~15
+    if (step != 1 and width > 1) or ld & 15 or ld < width or t.data_ptr() & 15:
         raise KernelError(f"{name}: rows of 8-bit integers are contiguous and start on 16 bytes (see q8_rows), got strides {t.stride()}")
-    if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] != rows or (scale.stride(0) != 1 and rows > 1):
+    if scale.dtype is not torch.float32 or scale.shape != (rows,) or (rows > 1 and scale.stride(0) != 1):
         raise KernelError(f"{name}: {rows} rows need as many float32 scales side by side, got {scale.dtype} {tuple(scale.shape)}")
-    return ld
+    return rows, width, ld
 
 
-def _plain_rows(t: torch.Tensor, name: str, shape) -> int:
+def _plain_rows(t: torch.Tensor, name: str, rows: int, width: int) -> int:
     """Checks a float32 or bfloat16 matrix with contiguous rows; the rows' distance."""
-    if t.dim() != 2 or t.shape != shape:
-        raise KernelError(f"{name} must be a {tuple(shape)} matrix, got {tuple(t.shape)}")
-    rows, width = t.shape
-    ld = t.stride(0) if rows > 1 else width
-    if (t.stride(1) != 1 and width > 1) or ld < width:
+    if t.shape != (rows, width):
+        raise KernelError(f"{name} must be a {(rows, width)} matrix, got {tuple(t.shape)}")
+    ld, step = t.stride()
+    if rows < 2:
+        ld = width
+    if (step != 1 and width > 1) or ld < width:
         raise KernelError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
     return ld
 
 
 def _on_current_device(what: str, *tensors) -> None:
     here = tensors[0].get_device()
-    if here < 0 or any(t is not None and t.get_device() != here for t in tensors) or here != torch._C._cuda_getDevice():
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            here = -1
+    if here < 0 or here != torch._C._cuda_getDevice():
         raise KernelError(f"{what}: all operands lie on the current CUDA device, got {', '.join(str(t.device) for t in tensors if t is not None)}")
 
 
@@ -2410,9 +2418,8 @@ def quantize_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor) -> None:
     """Rows of x (float32 or bfloat16 [rows, width]) as 8-bit integers with a scale each:  q = 127 x / max|x| rounded to the nearest whole
     number (ties to even, decided by the numbers as they are stored),  scale = max|x| / 127;  q * scale stands for x.  A row of zeros has the scale
     0, a row that holds a NaN or an infinity the scale NaN and zeros.  A weight matrix's rows are its output channels."""
-    ldq = _q8(q, scale, "q")
-    ldx = _plain_rows(x, "x", q.shape)
-    rows, width = q.shape
+    rows, width, ldq = _q8(q, scale, "q")
+    ldx = _plain_rows(x, "x", rows, width)
     code = dtype_code(x.dtype)
     if width == 0:
         raise KernelError("quantize_q8: rows without entries")
@@ -2424,9 +2431,8 @@ def quantize_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor) -> None:
 
 def dequantize_q8(out: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
     """out (float32 or bfloat16) = q * scale: what rows of 8-bit integers stand for."""
-    ldq = _q8(q, scale, "q")
-    ldy = _plain_rows(out, "out", q.shape)
-    rows, width = q.shape
+    rows, width, ldq = _q8(q, scale, "q")
+    ldy = _plain_rows(out, "out", rows, width)
     code = dtype_code(out.dtype)
     _on_current_device("dequantize_q8", out, q, scale)
     if rows == 0 or width == 0:
@@ -2438,16 +2444,15 @@ def rmsnorm_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, gain: torc
                total: torch.Tensor | None = None) -> None:
     """t = x + add in x's type (t = x without `add`);  q, scale = the 8-bit rows of rmsnorm(t) * gain (quantize_q8).  `total` receives t; it may be x
     itself: the residual's rows then take the addition in place.  The root mean square goes into the scale, so the integers are those of t * gain."""
-    ldq = _q8(q, scale, "q")
-    ldx = _plain_rows(x, "x", q.shape)
-    rows, width = q.shape
-    if gain.dim() != 1 or gain.shape[0] != width or (width > 1 and gain.stride(0) != 1):
+    rows, width, ldq = _q8(q, scale, "q")
+    ldx = _plain_rows(x, "x", rows, width)
+    if gain.shape != (width,) or (width > 1 and gain.stride(0) != 1):
         raise KernelError(f"rmsnorm_q8: the gain must hold {width} entries side by side, got {tuple(gain.shape)}")
     ldadd = ldt = 0
     if add is not None:
-        ldadd = _plain_rows(add, "add", q.shape)
+        ldadd = _plain_rows(add, "add", rows, width)
     if total is not None:
-        ldt = _plain_rows(total, "total", q.shape)
+        ldt = _plain_rows(total, "total", rows, width)
         if add is None or total.dtype != x.dtype:
             raise KernelError("rmsnorm_q8: `total` takes the sum of x and `add` in x's type")
     x_code, add_code, gain_code = dtype_code(x.dtype), dtype_code(add.dtype) if add is not None else F32, dtype_code(gain.dtype)
@@ -2466,12 +2471,12 @@ def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: tor
     in 32-bit integers, the rest in float32.  Store (float32 or bfloat16), accumulate (float32) or SwiGLU (w and w_scale have 2N rows, gates first;
     `glu` and `glu_bias` as for gemm_tc, with outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row.  `weights_settled`: w was complete before
     the kernel in front of this call was launched, as a model's weights are; it is then fetched while that one still runs."""
-    lda, ldw = _q8(a, a_scale, "a"), _q8(w, w_scale, "w")
-    T, K = a.shape
+    T, K, lda = _q8(a, a_scale, "a")
+    rows_w, inner, ldw = _q8(w, w_scale, "w")
     gated = epilogue == EPILOGUE_SWIGLU
-    N = w.shape[0] // 2 if gated else w.shape[0]
-    ldo = _plain_rows(out, "out", (T, N))
-    if w.shape[1] != K or (gated and w.shape[0] % 2) or not 0 < K <= Q8_MAX_INNER:
+    N = rows_w // 2 if gated else rows_w
+    ldo = _plain_rows(out, "out", T, N)
+    if inner != K or (gated and rows_w % 2) or not 0 < K <= Q8_MAX_INNER:
         raise KernelError(f"gemm_q8_tc: a {tuple(a.shape)} and w {tuple(w.shape)} do not go together (rows of equal length, 1 to {Q8_MAX_INNER} entries, "
                           f"gate and up rows of equal number)")
     if epilogue not in (EPILOGUE_STORE, EPILOGUE_ACCUMULATE, EPILOGUE_SWIGLU) or (epilogue == EPILOGUE_ACCUMULATE and out.dtype != torch.float32):

@@ -31,10 +31,7 @@ def _codes(x):
 
 def _fresh(rows, width, fill=77):
     """Room for rows with one row behind them, all bytes `fill`; (q, the whole buffer)."""
-    ops = _ops()
-    whole = ops.q8_rows(rows + 1, width, DEV)
-    whole = whole._base if whole._base is not None else whole
-    whole.fill_(fill)
+    whole = torch.full((rows + 1, -(-width // 16) * 16), fill, dtype=torch.int8, device=DEV)
     return whole[:rows, :width], whole
 
 
@@ -219,12 +216,9 @@ def test_norm_of_rows_without_numbers():
 
 # -- products -------------------------------------------------------------------------------------------------------------------
 def _operands(T, rows_w, K, seed=0):
-    ops = _ops()
     g = torch.Generator(device=DEV).manual_seed(seed + T * 3 + rows_w * 5 + K)
-    a, w = ops.q8_rows(T, K, DEV), ops.q8_rows(rows_w, K, DEV)
+    a, w = _fresh(T, K, 111)[0], _fresh(rows_w, K, 111)[0]       # (what lies between the rows is not zero)
     for m in (a, w):
-        whole = m._base if m._base is not None else m
-        whole.fill_(111)                            # what lies between the rows is not zero
         m.copy_(torch.randint(-128, 128, m.shape, generator=g, device=DEV, dtype=torch.int8))
     sa = torch.exp(torch.randn(T, generator=g, device=DEV)) * 0.02
     sw = torch.exp(torch.randn(rows_w, generator=g, device=DEV)) / (3000 * math.sqrt(K))
