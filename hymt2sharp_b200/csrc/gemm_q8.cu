@@ -154,6 +154,9 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const int my_blocks = max(0, min(num_k_blocks, kb_begin + p.k_blocks_per_split) - kb_begin);
     const int n0 = blockIdx.x * TILE_M, t0 = blockIdx.y * BN;
 
+    if (threadIdx.x == 32) {            // the maps are on their way while the barriers are made
+        for (const CUtensorMap* map : {&map_w, &map_a}) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory");
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; s++) {
             mbar_init(full0 + 8 * s, 1);
@@ -382,6 +385,9 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const int num_k_blocks = (p.K + BLOCK_K - 1) / BLOCK_K;
     const int tiles_t = (p.T + 2 * TILE_M - 1) / (2 * TILE_M), tiles_n = (p.N + OUT_COLS - 1) / OUT_COLS, num_tiles = tiles_t * tiles_n;
 
+    if (threadIdx.x == 32) {            // the maps are on their way while the barriers are made
+        for (const CUtensorMap* map : {&map_w, &map_a}) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory");
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; s++) {
             mbar_init(full0 + 8 * s, 1);
@@ -499,14 +505,28 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if constexpr (GATED) tmem_load_two<PIECE>(lane_addr + c, lane_addr + bn / 2 + c, y, u);
                 else if constexpr (PIECE == 32) tmem_load32(lane_addr + c, y);
                 else tmem_load16(lane_addr + c, y);
-                const float ws_now = ws, us_now = us;
+                // the piece's scales go round the warp through the buffer that its output will fill (32 shuffles a piece took longer than the products);
+                // TMA has read what lay there two pieces ago
+                const uint32_t out = stage_out + (used & 1) * OUT_BUFFER;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                __syncwarp();
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(out + lane * 4), "f"(ws) : "memory");
+                if constexpr (GATED) asm volatile("st.shared.f32 [%0], %1;" ::"r"(out + 128 + lane * 4), "f"(us) : "memory");
+                __syncwarp();
                 ws = column_scale(tile, c + 2 * PIECE, 0);
                 if constexpr (GATED) us = column_scale(tile, c + 2 * PIECE, 1);
+                auto scale_all = [&](float* v, uint32_t at) {
 #pragma unroll
-                for (int q = 0; q < PIECE; q++) y[q] = scaled(__float_as_int(y[q]), sa, __shfl_sync(0xffffffffu, ws_now, q));
+                    for (int q = 0; q < PIECE; q += 4) {
+                        float s4[4];
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(s4[0]), "=f"(s4[1]), "=f"(s4[2]), "=f"(s4[3]) : "r"(at + q * 4) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[q + i] = scaled(__float_as_int(v[q + i]), sa, s4[i]);
+                    }
+                };
+                scale_all(y, out);
                 if constexpr (GATED) {
-#pragma unroll
-                    for (int q = 0; q < PIECE; q++) u[q] = scaled(__float_as_int(u[q]), sa, __shfl_sync(0xffffffffu, us_now, q));
+                    scale_all(u, out + 128);
                     if (plain) {
 #pragma unroll
                         for (int q = 0; q < PIECE; q++) y[q] = swish(y[q], 1.0f) * u[q];
@@ -516,9 +536,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                 }
                 if (p.tma_out) {
-                    // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them; the buffer of two pieces ago has been read
-                    const uint32_t out = stage_out + (used & 1) * OUT_BUFFER;
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them
                     __syncwarp();
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
@@ -675,7 +693,7 @@ Plan make_plan(int T, int N, int K, bool gated, int sm_count) {
                 if (plan_few(pl, T, N, K, gated, sm_count, bn, splits) && pl.cost < best.cost) best = pl;
     }
     if (T > 64)
-        for (int bn = PAIR_BN; bn >= 64; bn -= 64) {
+        for (int bn = PAIR_BN; bn >= 64; bn -= gated ? 64 : 32) {      // (a piece of 32 output columns at a time)
             plan_pairs(pl, T, N, K, gated, sm_count, bn);
             if (pl.cost < best.cost) best = pl;
         }

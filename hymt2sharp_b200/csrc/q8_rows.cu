@@ -211,8 +211,8 @@ template <bool WARP, bool SUM> __device__ __forceinline__ void over_row(float& m
 template <typename TX, int CH, bool WARP, bool VEC>
 __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, WARP ? 1 : CH == 4 && sizeof(TX) == 2 ? 3 : VEC ? 2 : 1) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
     __shared__ float2 scratch[32];
+    pdl_wait();      // (then release: the kernel in front may be one that has yet to take its tensor memory, which the one behind must not take first)
     pdl_launch_dependents();
-    pdl_wait();
     const Place<WARP> at(rows);
     if (!at.in) return;
     const TX* src = x + at.row * ldx;
@@ -288,8 +288,8 @@ constexpr int LONGEST_HELD = 16384;
 template <typename TX, bool VEC>
 __global__ void __launch_bounds__(1024) quantize_q8_long_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int width) {
     __shared__ float2 scratch[32];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const TX* src = x + (size_t)blockIdx.x * ldx;
     float most = 0.f, none = 0.f;
     for (int c = 0; c * 8192 < width; c++) {

@@ -104,5 +104,5 @@ def test_plans_stay_within_the_machine(gated):
                         assert p["shared_bytes"] >= max(p["stages"] * stage, sums) + 1024 and p["shared_bytes"] <= 226 * 1024
                         assert p["ctas"] == -(-N // 128) * -(-T // p["width"]) * p["splits"]
                     else:
-                        assert T > 64 and p["splits"] == 1 and p["width"] in (64, 128, 192, 256) and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= sms
+                        assert T > 64 and p["splits"] == 1 and 64 <= p["width"] <= 256 and p["width"] % (64 if gated else 32) == 0 and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= sms
                         assert p["stages"] * (16384 + p["width"] * 64) + 32768 + 1024 == p["shared_bytes"] <= 226 * 1024
