@@ -2443,7 +2443,8 @@ def dequantize_q8(out: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> No
 def rmsnorm_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, gain: torch.Tensor, eps: float, add: torch.Tensor | None = None,
                total: torch.Tensor | None = None) -> None:
     """t = x + add in x's type (t = x without `add`);  q, scale = the 8-bit rows of rmsnorm(t) * gain (quantize_q8).  `total` receives t; it may be x
-    itself: the residual's rows then take the addition in place.  The root mean square goes into the scale, so the integers are those of t * gain."""
+    itself: the residual's rows then take the addition in place.  The root mean square goes into the scale, so the integers are those of t * gain in float32
+    (entries of x beyond 1e19 have squares that float32 does not hold, and the scale becomes 0)."""
     rows, width, ldq = _q8(q, scale, "q")
     ldx = _plain_rows(x, "x", rows, width)
     if gain.shape != (width,) or (width > 1 and gain.stride(0) != 1):
@@ -2468,9 +2469,11 @@ def rmsnorm_q8(q: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, gain: torc
 def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int, status: torch.Tensor,
                glu: GluRule | None = None, glu_bias: torch.Tensor | None = None, weights_settled: bool = False) -> None:
     """out[t, n] = epilogue(a_scale[t] * w_scale[n] * sum_k a[t, k] * w[n, k]): 8-bit rows of tokens with 8-bit rows of weights, the sums exact
-    in 32-bit integers, the rest in float32.  Store (float32 or bfloat16), accumulate (float32) or SwiGLU (w and w_scale have 2N rows, gates first;
-    `glu` and `glu_bias` as for gemm_tc, with outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row.  `weights_settled`: w was complete before
-    the kernel in front of this call was launched, as a model's weights are; it is then fetched while that one still runs."""
+    in 32-bit integers, the rest in float32: a row is the same bit for bit whatever other rows there are (a sum below 2^-126 may come out as 0 where it is
+    added).  Store (float32 or bfloat16), accumulate (float32) or SwiGLU (w and w_scale have 2N rows, gates first; `glu` and `glu_bias` as for gemm_tc, with
+    outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row; `out` shares no memory with the operands.
+    `weights_settled`: w was complete before the kernel in front of this call was launched, as a model's weights are; it is then fetched while that one
+    still runs."""
     T, K, lda = _q8(a, a_scale, "a")
     rows_w, inner, ldw = _q8(w, w_scale, "w")
     gated = epilogue == EPILOGUE_SWIGLU
@@ -2481,7 +2484,7 @@ def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: tor
                           f"gate and up rows of equal number)")
     if epilogue not in (EPILOGUE_STORE, EPILOGUE_ACCUMULATE, EPILOGUE_SWIGLU) or (epilogue == EPILOGUE_ACCUMULATE and out.dtype != torch.float32):
         raise KernelError(f"gemm_q8_tc: epilogue {epilogue} into {out.dtype} is not built (sums are added into float32)")
-    if status.dtype != torch.int32:
+    if status.dtype != torch.int32 or status.numel() == 0:
         raise KernelError("gemm_q8_tc: the status word is an int32 tensor")
     code = dtype_code(out.dtype)
     _on_current_device("gemm_q8_tc", out, a, a_scale, w, w_scale, status, glu_bias)
@@ -2500,3 +2503,39 @@ def gemm_q8_describe(tokens: int, out_features: int, inner: int, gated: bool, sm
     out = (c_long * 7)()
     _check(_lib().hymt2_gemm_q8_describe(c_int(tokens), c_int(out_features), c_int(inner), c_int(bool(gated)), c_int(sm_count), out), "gemm_q8_describe", 0)
     return dict(zip(("few", "width", "stages", "splits", "k_blocks", "ctas", "shared_bytes"), out))
+
+
+class _DenseBlockQ8(ctypes.Structure):
+    """csrc/dense_block_q8.cu: Hymt2DenseBlockQ8, in the order of its members."""
+    _fields_ = ([(n, c_void_p) for n in ("residual", "w_qkv", "w_o", "w_gate_up", "w_down", "s_qkv", "s_o", "s_gate_up", "s_down", "norm1_gain", "norm2_gain",
+                                         "q_gain", "k_gain", "glu_bias", "x8", "att8", "act8", "x_scale", "att_scale", "act_scale", "qkv", "q", "att", "added",
+                                         "act", "k_plane", "v_plane", "block_table", "token_seq", "token_pos", "slot_ids", "cu_seqlens", "kv_lens", "inv_freq",
+                                         "status")]
+                + [(n, c_long) for n in ("cache_blocks", "ld_qkv", "ld_o", "ld_gate_up", "ld_down")]
+                + [(n, c_int) for n in ("T", "hidden", "inner", "nh", "nkv", "d", "batch", "max_new_tokens", "table_stride", "block_tokens", "rope_dim",
+                                        "write_kv", "window", "gain_dtype", "norm1_dtype", "norm2_dtype", "glu_kind")]
+                + [(n, c_float) for n in ("qk_eps", "norm1_eps", "norm2_eps", "scale", "glu_limit", "glu_alpha")])
+
+
+def dense_block_q8_fits() -> bool:
+    """Whether the arguments are laid out as the library has them."""
+    return _lib().hymt2_dense_block_q8_bytes() == ctypes.sizeof(_DenseBlockQ8)
+
+
+def dense_block_q8(residual, w_qkv, w_o, w_gate_up, w_down, norm1, norm2, q_gain, k_gain, glu: GluRule | None, glu_bias, space, k_plane, v_plane, block_table,
+                   ctx, inv_freq, rope_dim: int, nh: int, nkv: int, d: int, inner: int, write_kv: bool, window: int, qk_eps: float, scale: float) -> None:
+    """The ten kernels of a dense block's prompt step with 8-bit weights (parts.dense, which has checked the operands): w_*: parts.linear8.Rows8; `space`: the
+    8-bit rows (x, att, act) with their scales and the bfloat16 buffers (qkv, q, att, added, act) that the kernels hand on."""
+    T, hidden = residual.shape
+    (x8, att8, act8), (qkv, q, att, added, act) = space
+    if (q_gain is None) != (k_gain is None) or (q_gain is not None and (q_gain.dtype != k_gain.dtype or q_gain.numel() != d or k_gain.numel() != d)):
+        raise KernelError(f"dense_block_q8: the gains of q and k hold {d} entries of one type each")
+    a, weights, glu = _address, (w_qkv, w_o, w_gate_up, w_down), glu or GLU_SILU
+    block = _DenseBlockQ8(
+        a(residual), *(a(w.q) for w in weights), *(a(w.scale) for w in weights), a(norm1.gain), a(norm2.gain), a(q_gain), a(k_gain), a(glu_bias),
+        a(x8.q), a(att8.q), a(act8.q), a(x8.scale), a(att8.scale), a(act8.scale), a(qkv), a(q), a(att), a(added), a(act), a(k_plane), a(v_plane),
+        a(block_table), a(ctx.token_seq), a(ctx.token_pos), a(ctx.slot_ids), a(ctx.cu_seqlens), a(ctx.kv_lens), a(inv_freq), a(ctx.status),
+        k_plane.shape[0], *(w.q.stride(0) for w in weights), T, hidden, inner, nh, nkv, d, ctx.num_seqs, ctx.max_new_tokens, block_table.stride(0),
+        k_plane.shape[2], rope_dim, 1 if write_kv else 0, window, dtype_code(q_gain.dtype) if q_gain is not None else F32, dtype_code(norm1.gain.dtype),
+        dtype_code(norm2.gain.dtype), GLU_KINDS[glu.kind], qk_eps, norm1.eps, norm2.eps, scale, glu.limit, glu.alpha)
+    _check(_lib().hymt2_dense_block_q8(ctypes.byref(block), _stream()), "dense_block_q8", 10, timed=False)

@@ -21,7 +21,7 @@ class PreNormBlock:
         self.mixer = build_part("mixer", mixer)
         self.norm2 = build_part("norm", norm2)
         self.feed_forward = build_part("feed_forward", feed_forward)
-        self.dense = dense.takes(self)         # whether a prompt's step may be launched by one call
+        self.dense, self.dense_rows8 = dense.takes(self), dense.takes_rows8(self)     # whether a prompt's step may be launched by one call
 
     def parts(self):
         return (self.norm1, self.mixer, self.norm2, self.feed_forward)
@@ -53,6 +53,8 @@ class PreNormBlock:
         return self.norm1 if getattr(self.mixer, "takes_prenormed", False) else None
 
     def forward(self, residual, ctx, slots) -> None:
+        if self.dense_rows8 and dense.try_block_rows8(self, residual, ctx, slots[0]):
+            return
         if makes_rows8(self.norm1, self.mixer):
             x = self.norm1.rows8(residual, ctx)
         else:

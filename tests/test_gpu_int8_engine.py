@@ -109,6 +109,31 @@ def test_generation_through_graphs_is_generation_step_by_step(name, dtype, model
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name, one_call", [("M", True), ("H", True), ("HW", True), ("B", False)])
+def test_a_prompts_block_by_one_call_is_its_parts_one_by_one(name, one_call, model_dirs, monkeypatch):
+    """Heads of 64 and 128, with and without a window, prompts and a further piece of one: logits and the number of launches."""
+    from hymt2sharp_b200 import StepEntry
+    from hymt2sharp_b200.kernels import ops
+    eng = _engine(model_dirs(name), "bfloat16", max_batch=2)
+    calls, launch = [], ops.dense_block_q8
+    monkeypatch.setattr(ops, "dense_block_q8", lambda *args: (calls.append(1), launch(*args)))
+    seqs = [helpers.random_tokens(eng.vocab, n, n) for n in (203, 31)]
+    results = []
+    for whole in (True, False):
+        for block in eng.model.blocks:
+            block.dense_rows8 = block.dense_rows8 and whole
+        slots, before, logits = eng.alloc_slots(2), ops.launches, []
+        for cut in (slice(0, 20), slice(20, 203)):
+            entries = [StepEntry(s, q[cut], list(range(len(q[cut])))) for s, q in zip(slots, seqs)]
+            logits.append(eng.step(entries).clone())
+        results.append((torch.cat(logits), ops.launches - before, len(calls)))
+        eng.free_slots(slots)
+    eng.check()
+    (a, na, ca), (b, nb, cb) = results
+    assert torch.equal(a, b) and na == nb and ca == (2 * len(eng.model.blocks) if one_call else 0) and cb == ca
+
+
+@pytest.mark.gpu
 def test_the_layers_matrices_are_held_once_and_in_8_bits(model_dirs):
     from hymt2sharp_b200 import Engine
     stored, small = Engine(model_dirs("H"), dtype="bfloat16", max_tokens=256), _engine(model_dirs("H"), "bfloat16", max_tokens=256)

@@ -453,3 +453,54 @@ def test_a_feed_forward_as_a_layer_runs_it(T):
         torch.cuda.synchronize()
         assert torch.equal(gx, x) and torch.equal(gact, act) and torch.equal(gout, out)
     assert status.tolist() == [0, 0, 0, 0]
+
+
+def test_offsets_beyond_32_bits():
+    """Matrices of more than 2^31 entries: their last rows."""
+    ops = _ops()
+    status = torch.zeros(4, dtype=torch.int32, device=DEV)
+    rows, width = 36000, 60000
+    x = torch.zeros(rows, width, dtype=BF, device=DEV)
+    x[-3:] = _x(3, width, BF)
+    q, s = ops.q8_rows(rows, width, DEV), torch.empty(rows, device=DEV)
+    ops.quantize_q8(q, s, x)
+    want_q, want_s = _codes(x[-3:].double())
+    assert torch.equal(q[-3:], want_q) and not q[:-3].any() and not s[:-3].any()
+    _same_scale(s[-3:], want_s)
+    ops.dequantize_q8(x, q, s)
+    assert torch.equal(x[-3:], (q[-3:].float() * s[-3:, None]).bfloat16())
+    gain = torch.ones(width, device=DEV)
+    ops.rmsnorm_q8(q, s, x, gain, 1e-5, add=x, total=x)
+    want_q = _codes((2 * (want_q.float() * want_s.float()[:, None]).bfloat16().double()))[0]
+    assert torch.equal(q[-3:], want_q)
+    del x, q
+    T, N, K = 70000, 32768, 64
+    a, sa, w, sw = _operands(T, N, K)
+    for dtype, epilogue in ((BF, ops.EPILOGUE_STORE), (F32, ops.EPILOGUE_ACCUMULATE)):
+        out = torch.zeros(T, N, dtype=dtype, device=DEV)
+        ops.gemm_q8_tc(out, a, sa, w, sw, epilogue, status)
+        want = (a[-40:].double() @ w.double().T) * sa[-40:].double()[:, None] * sw.double()
+        assert ((out[-40:].double() - want).abs() <= (_half_step(dtype) * 1.01 + 4 * U) * want.abs()).all()
+        del out
+    assert status.tolist() == [0, 0, 0, 0]
+
+
+def test_weights_made_by_the_kernel_in_front():
+    """Rows that become integers just in front of the product that takes them as its weights, again and again over the same buffers: a product fetches its
+    weights ahead of the kernel in front only where the caller says that they were there before."""
+    ops = _ops()
+    status = torch.zeros(4, dtype=torch.int32, device=DEV)
+    for T, N, K in ((3, 2048, 4096), (600, 4096, 2048)):
+        a, sa, _, _ = _operands(T, 1, K)
+        w, sw = ops.q8_rows(N, K, DEV), torch.empty(N, device=DEV)
+        xs = [torch.randn(N, K, device=DEV).bfloat16() for _ in range(4)]
+        outs = [torch.empty(T, N, device=DEV) for _ in xs]
+        for x, out in zip(xs, outs):
+            ops.quantize_q8(w, sw, x)
+            ops.gemm_q8_tc(out, a, sa, w, sw, ops.EPILOGUE_STORE, status)
+        torch.cuda.synchronize()
+        for x, out in zip(xs, outs):
+            q, s = _codes(x.double())
+            want = (a.double() @ q.double().T) * sa.double()[:, None] * s
+            assert ((out.double() - want).abs() <= 6 * U * want.abs()).all()
+    assert status.tolist() == [0, 0, 0, 0]
