@@ -158,10 +158,11 @@ class GQAAttention:
                         ctx.slot_ids, epilogue.inv_freq, epilogue.rope_dim, self.q_gain, self.k_gain, self.eps, nh, nkv, d)
         out = torch.empty((T, nh * d), dtype=q.dtype, device=q.device)
         self.attend(out, q, k_plane, v_plane, block_table, ctx)
-        if ctx.decode and ctx.weights_ahead is not None:
+        if ctx.decode and ctx.weights_ahead is not None and self.weights is None:
             # the feed-forward's first weights come into L2 beside the output projection and the norm, which leave
             # the memory idle; the request starts once the attention is through (not earlier: its last loads and
-            # the folding of its partials are sensitive to traffic)
+            # the folding of its partials are sensitive to traffic).  A product with 8-bit weights fetches its own ahead of the kernel in
+            # front, and the branch beside it cost such a step 1 to 4 %.
             ops.prefetch_beside(ctx.weights_ahead)
         if store:
             self.out_store(out, out=residual)
