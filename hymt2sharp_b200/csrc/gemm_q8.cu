@@ -486,7 +486,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         float sa_next = token_scale(pair), ws_next = column_scale(pair, side * PIECE, 0), us_next = GATED ? column_scale(pair, side * PIECE, 1) : 0.f;
         for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
             const int buf = j & 1;
-            const int t_first = first_token(tile), t = t_first + lane;
+            const int t_first = first_token(tile);
             const int n_first = (tile / tiles_t) * OUT_COLS;
             const float sa = sa_next;
             float ws = ws_next, us = us_next;
@@ -535,25 +535,25 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         for (int q = 0; q < PIECE; q++) y[q] = n + q < p.N ? gated_at(p.glu, y[q], u[q], n + q, p.N) : 0.f;
                     }
                 }
-                if (p.tma_out) {
-                    // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them
-                    __syncwarp();
+                // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them
+                __syncwarp();
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const uint32_t at = out + lane * PIECE_BYTES + ((q ^ ((lane >> 1) & 3)) << 4);
-                        uint32_t w[4];
-                        if constexpr (sizeof(TC) == 4) {
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t at = out + lane * PIECE_BYTES + ((q ^ ((lane >> 1) & 3)) << 4);
+                    uint32_t w[4];
+                    if constexpr (sizeof(TC) == 4) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) w[i] = __float_as_uint(y[4 * q + i]);
-                        } else {
+                        for (int i = 0; i < 4; i++) w[i] = __float_as_uint(y[4 * q + i]);
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(y[8 * q + 2 * i], y[8 * q + 2 * i + 1]);
-                                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
+                        for (int i = 0; i < 4; i++) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(y[8 * q + 2 * i], y[8 * q + 2 * i + 1]);
+                            w[i] = *reinterpret_cast<const uint32_t*>(&h);
                         }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                     }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                }
+                if (p.tma_out) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) {
@@ -566,11 +566,26 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                     used++;
-                } else if (t < p.T) {
-                    TC* dst = C + (size_t)t * p.ldc + n;
-#pragma unroll
-                    for (int q = 0; q < PIECE; q++)
-                        if (n + q < p.N) dst[q] = from_float<TC>(EPI == EPI_ACCUMULATE ? __fadd_rn(to_float(dst[q]), y[q]) : y[q]);
+                } else {
+                    // rows that TMA does not write: a row's columns side by side, so that an access meets a few sectors and not 32
+                    __syncwarp();
+                    const int col = lane % PIECE, at = col * (int)sizeof(TC);
+#pragma unroll 4
+                    for (int row = lane / PIECE; row < 32; row += 32 / PIECE) {
+                        const uint32_t from = out + row * PIECE_BYTES + ((((at >> 4) ^ ((row >> 1) & 3)) << 4) | (at & 15));
+                        if (t_first + row < p.T && n + col < p.N) {
+                            TC* dst = C + (size_t)(t_first + row) * p.ldc + n + col;
+                            if constexpr (sizeof(TC) == 4) {
+                                float v;
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+                                *dst = EPI == EPI_ACCUMULATE ? __fadd_rn(*dst, v) : v;
+                            } else {
+                                unsigned short v;
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+                                *dst = __ushort_as_bfloat16(v);
+                            }
+                        }
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
