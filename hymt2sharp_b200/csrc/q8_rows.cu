@@ -5,14 +5,15 @@
 //   rmsnorm_q8      t = x + add (kept in x's type), r = 1 / sqrt(mean(t^2) + eps): q and s of the rows t gain, s times r.  r is the same for
 //                   the whole row, so it changes no integer and goes into the scale.
 // A row that holds a NaN or an infinity gets the scale NaN and zeros: whatever is computed from it is NaN.  A row of zeros gets the scale 0.
-// The whole numbers are exact: the quotient of the numbers as they are stored, not of rounded ones, decides (q8_settle).
+// The whole numbers are exact: the quotient of the numbers as they are stored, not of rounded ones, decides (q8_of).
 #include "common.cuh"
 
+// Each kernel waits for the one in front before it releases the one behind it: that one may take tensor memory which one in front has yet to take.
 namespace {
 
 struct RowCode {
     float f, inv, low, top;   // a power of two that keeps what follows in range; about 127 / (max|x| f), and what that leaves of it; max|x| f
-    bool none;            // zeros: nothing in the row, or nothing that is a number
+    bool none;                // zeros: nothing in the row, or nothing that is a number
 };
 
 // `top`: the largest |x|, infinity and NaN included
@@ -29,9 +30,9 @@ __device__ __forceinline__ RowCode row_code(float top) {
 }
 __device__ __forceinline__ float row_scale(float top) { return top < __uint_as_float(0x7f800000u) ? top / 127.0f : __uint_as_float(0x7fc00000u); }
 
-// x inv is within 127 (2^-23 + 2^-24) = 2.3e-5 of the quotient 127 x / top (the approximate reciprocal's last place, a rounding), so the nearest whole number r of the one is that of the other unless the quotient
-// lies within 3e-5 of a border b (a whole number and a half).  There the sign of 127 x - b top decides: 127 x is hi + lo without an error, hi - b top is
-// a multiple of half of top's last place and small, so both differences are exact.
+// x inv is within 127 (2^-23 + 2^-24) = 2.3e-5 of the quotient 127 x / top (the approximate reciprocal's last place, a rounding), so the nearest whole
+// number r of the one is that of the other unless the quotient lies within 3e-5 of a border b (a whole number and a half).  There the sign of
+// 127 x - b top decides: 127 x is hi + lo without an error, hi - b top is a multiple of half of top's last place and small, so both differences are exact.
 constexpr float NEAR_BORDER = 0.49997f;
 // Adding 1.5 * 2^23 rounds to a whole number (ties to even), whose two's complement then fills the lowest bits.
 constexpr float WHOLE = 12582912.0f;
@@ -208,10 +209,12 @@ template <bool WARP, bool SUM> __device__ __forceinline__ void over_row(float& m
     if (SUM) ss = warp_sum(mine.y);
 }
 
+// (blocks an SM: with 39 registers a thread one block of 896 was there at a time, and 8,192 x 14,336 took 179 us for 106 with two)
 template <typename TX, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, WARP ? 1 : CH == 4 && sizeof(TX) == 2 ? 3 : VEC ? 2 : 1) quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
+__global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, WARP ? 1 : CH == 4 && sizeof(TX) == 2 ? 3 : VEC ? 2 : 1)
+quantize_q8_kernel(int8_t* q, long ldq, float* scale, const TX* x, long ldx, int rows, int width) {
     __shared__ float2 scratch[32];
-    pdl_wait();      // (then release: the kernel in front may be one that has yet to take its tensor memory, which the one behind must not take first)
+    pdl_wait();
     pdl_launch_dependents();
     const Place<WARP> at(rows);
     if (!at.in) return;
@@ -247,8 +250,8 @@ struct NormQ8Params {
 template <typename TX, typename TA, typename TG, int CH, bool WARP, bool VEC>
 __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP && CH == 1 && VEC ? 2 : 1) rmsnorm_q8_kernel(NormQ8Params p) {
     __shared__ float2 scratch[32];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const Place<WARP> at(p.rows);
     if (!at.in) return;
     float v[CH][8], most = 0.f, ss = 0.f;
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP && CH == 1 && VEC ? 2
             float a[8];
             load8<VEC>((const TA*)p.add + at.row * p.ldadd, c, at.tid, at.threads, p.width, a);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[c][i] = to_float(from_float<TX>(v[c][i] + a[i]));   // the sum as the rows are kept: what is normed is what a later reader finds
+            for (int i = 0; i < 8; i++) v[c][i] = to_float(from_float<TX>(v[c][i] + a[i]));   // (as the rows are kept: what a later reader finds is normed)
             if (p.total) store8<VEC>((TX*)p.total + at.row * p.ldt, c, at.tid, at.threads, p.width, v[c]);
         }
     }
@@ -311,8 +314,8 @@ __global__ void __launch_bounds__(1024) quantize_q8_long_kernel(int8_t* q, long 
 template <typename TX, typename TA, typename TG, bool VEC>
 __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(NormQ8Params p) {
     __shared__ float2 scratch[32];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const size_t r = blockIdx.x;
     const TX* x = (const TX*)p.x + r * p.ldx;
     const TA* add = p.add ? (const TA*)p.add + r * p.ldadd : nullptr;
@@ -353,8 +356,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(NormQ8Params p) {
 template <typename TY, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_q8_kernel(TY* y, long ldy, const int8_t* q, long ldq, const float* scale, int rows, int width, int pieces) {
     constexpr int V = VEC ? 16 / (int)sizeof(TY) : 1, STEP = 4 * 32 * V * (VEC ? 1 : 4);
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const long all = (long)rows * pieces, step = (long)gridDim.x * (blockDim.x >> 5);
     for (long i = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < all; i += step) {
@@ -390,13 +393,15 @@ __global__ void __launch_bounds__(256) dequantize_q8_kernel(TY* y, long ldy, con
 
 inline bool whole(const void* p, long ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
 
-// How a row is shared: groups of 8 entries a thread, a warp or a block a row, threads of a block.
+// How a row is shared: groups of 8 entries a thread, a warp or a block a row, threads of a block.  Four groups a thread where there are more rows than two blocks an
+// SM, so that what a thread does once a row costs less (8,192 x 14,336 bfloat16 69 us, with two groups 91); fewer where a row's own way counts (64 x 4,096 1.7 us
+// with one group, 2.2 with two).  A norm stays with one group as far as 1,024 threads go (8,192 x 4,096 57 us, with two groups 62).
 struct Share { int ch, threads, blocks; bool warp; };
 constexpr int FEW_ROWS = 296;
 Share share_of(int rows, int width, bool norm, bool vec) {
     const int groups = (width + 7) / 8;
     if (groups <= 128) return Share{groups <= 32 ? 1 : groups <= 64 ? 2 : 4, 256, (rows + 7) / 8, true};
-    // (a norm's sums are added in an order that the share decides, so its share hangs on the width alone)
+    // (a norm's sums are added in an order that the share decides, so its share hangs on the width, and on whether rows start on 16 bytes, alone)
     const int ch = !norm && vec && rows > FEW_ROWS ? 4 : groups <= 1024 ? 1 : 2;
     return Share{ch, ((groups + ch - 1) / ch + 31) / 32 * 32, rows, false};
 }

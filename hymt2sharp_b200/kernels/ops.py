@@ -2517,9 +2517,15 @@ class _DenseBlockQ8(ctypes.Structure):
                 + [(n, c_float) for n in ("qk_eps", "norm1_eps", "norm2_eps", "scale", "glu_limit", "glu_alpha")])
 
 
+_dense_q8_fits = None
+
+
 def dense_block_q8_fits() -> bool:
     """Whether the arguments are laid out as the library has them."""
-    return _lib().hymt2_dense_block_q8_bytes() == ctypes.sizeof(_DenseBlockQ8)
+    global _dense_q8_fits
+    if _dense_q8_fits is None:
+        _dense_q8_fits = _lib().hymt2_dense_block_q8_bytes() == ctypes.sizeof(_DenseBlockQ8)
+    return _dense_q8_fits
 
 
 def dense_block_q8(residual, w_qkv, w_o, w_gate_up, w_down, norm1, norm2, q_gain, k_gain, glu: GluRule | None, glu_bias, space, k_plane, v_plane, block_table,
