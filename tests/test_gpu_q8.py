@@ -122,6 +122,48 @@ def test_rows_of_wider_buffers_and_odd_addresses(dtype):
         assert torch.equal(q, want_q) and torch.equal(total[:, :width], x) and (total[:, width:] == 3.0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("width", [1, 3, 8, 17, 41, 255, 263, 777, 1023, 1033, 4111, 9001, 17001, 33001])
+def test_rows_that_begin_anywhere(width, dtype):
+    """Every place of a row's begin within 16 bytes (rows of odd length have them all), what lies around the rows untouched, the sums in place."""
+    ops = _ops()
+    rows = 11
+    for offset, step in ((0, width), (1, width + 1), (2, width + 2), (3, width), (5, width + 7)):
+        def buffer(kind, fill):
+            flat = torch.full((rows * step + offset + 8,), fill, dtype=kind, device=DEV)
+            return flat, flat[offset:offset + rows * step].view(rows, step)[:, :width]
+
+        def around(flat, fill):
+            mask = torch.ones(flat.numel(), dtype=torch.bool, device=DEV)
+            mask[offset:offset + rows * step].view(rows, step)[:, :width] = False
+            return bool((flat[mask] == fill).all())
+        flat_x, x = buffer(dtype, 5.0)
+        x.copy_(_x(rows, width, dtype, offset))
+        q, whole = _fresh(rows, width)
+        s = torch.empty(rows, device=DEV)
+        ops.quantize_q8(q, s, x)
+        want_q, want_s = _codes(x.double())
+        assert torch.equal(q, want_q) and _untouched(whole, rows, width)
+        _same_scale(s, want_s)
+        flat_y, y = buffer(dtype, 3.0)
+        ops.dequantize_q8(y, q, s)
+        assert torch.equal(y, (q.float() * s[:, None]).to(dtype)) and around(flat_y, 3.0)
+        flat_a, a = buffer(BF if offset % 2 else F32, 9.0)
+        a.copy_(_x(rows, width, a.dtype, 40 + offset))
+        gain = (1 + 0.2 * torch.randn(width + offset, device=DEV)).to(dtype)[offset:]
+        t = (x.float() + a.float()).to(dtype)
+        want_q = _codes((t.float() * gain.float()).double())[0]
+        flat_t, total = buffer(dtype, 4.0)
+        s2 = torch.empty(rows, device=DEV)
+        ops.rmsnorm_q8(q, s, x, gain, 1e-5, add=a, total=total)
+        assert torch.equal(q, want_q) and torch.equal(total, t) and around(flat_t, 4.0)
+        ops.rmsnorm_q8(q, s2, x, gain, 1e-5, add=a, total=x)
+        assert torch.equal(q, want_q) and torch.equal(x, t) and around(flat_x, 5.0) and torch.equal(s, s2)
+        # the sums are added in the same order wherever a row begins
+        ops.rmsnorm_q8(q, s2, t.contiguous(), gain.clone(), 1e-5)
+        assert torch.equal(q, want_q) and torch.equal(s, s2)
+
+
 @pytest.mark.parametrize("width", [5, 64, 1024, 4096])
 def test_borders_between_whole_numbers(width):
     """Entries exactly half way between two whole numbers go to the even one, their neighbours in float32 to their own side."""
