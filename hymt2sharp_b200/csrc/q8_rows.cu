@@ -530,11 +530,13 @@ int run_norm(const Share& s, const NormQ8Params& p, cudaStream_t stream) {
     return hymt2_check_launch("rmsnorm_q8");
 }
 
+constexpr int MOST_Q8 = 1 << 28;        // rows, entries of a row: a row's bytes are counted in an int
+
 }  // namespace
 
 HYMT2_API int hymt2_quantize_q8(void* q, long ldq, float* scale, const void* x, int x_dtype, long ldx, int rows, int width, cudaStream_t stream) {
     if (rows == 0) return HYMT2_OK;
-    HYMT2_REQUIRE(rows > 0 && width > 0 && ldq >= width && ldx >= width, "quantize_q8: bad sizes rows=%d width=%d", rows, width);
+    HYMT2_REQUIRE(rows > 0 && rows <= MOST_Q8 && width > 0 && width <= MOST_Q8 && ldq >= width && ldx >= width, "quantize_q8: bad sizes rows=%d width=%d", rows, width);
     HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "quantize_q8: rows of integers must start on 16 bytes");
     HYMT2_DISPATCH_DTYPE(x_dtype, TX, {
         const bool shift = !whole(x, ldx, sizeof(TX));
@@ -551,7 +553,7 @@ HYMT2_API int hymt2_quantize_q8(void* q, long ldq, float* scale, const void* x, 
 
 HYMT2_API int hymt2_dequantize_q8(void* y, int y_dtype, long ldy, const void* q, long ldq, const float* scale, int rows, int width, cudaStream_t stream) {
     if (rows == 0) return HYMT2_OK;
-    HYMT2_REQUIRE(rows > 0 && width > 0 && ldq >= width && ldy >= width, "dequantize_q8: bad sizes rows=%d width=%d", rows, width);
+    HYMT2_REQUIRE(rows > 0 && rows <= MOST_Q8 && width > 0 && width <= MOST_Q8 && ldq >= width && ldy >= width, "dequantize_q8: bad sizes rows=%d width=%d", rows, width);
     HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "dequantize_q8: rows of integers must start on 16 bytes");
     HYMT2_DISPATCH_DTYPE(y_dtype, TY, {
         const bool shift = !whole(y, ldy, sizeof(TY));
@@ -568,7 +570,7 @@ HYMT2_API int hymt2_dequantize_q8(void* y, int y_dtype, long ldy, const void* q,
 HYMT2_API int hymt2_rmsnorm_q8(void* q, long ldq, float* scale, const void* x, int x_dtype, long ldx, const void* add, int add_dtype, long ldadd,
                                void* total, long ldt, const void* gain, int gain_dtype, int rows, int width, float eps, cudaStream_t stream) {
     if (rows == 0) return HYMT2_OK;
-    HYMT2_REQUIRE(rows > 0 && width > 0 && ldq >= width && ldx >= width, "rmsnorm_q8: bad sizes rows=%d width=%d", rows, width);
+    HYMT2_REQUIRE(rows > 0 && rows <= MOST_Q8 && width > 0 && width <= MOST_Q8 && ldq >= width && ldx >= width, "rmsnorm_q8: bad sizes rows=%d width=%d", rows, width);
     HYMT2_REQUIRE((uintptr_t)q % 16 == 0 && ldq % 16 == 0, "rmsnorm_q8: rows of integers must start on 16 bytes");
     HYMT2_REQUIRE(!total || add, "rmsnorm_q8: the sums have a place, but nothing is added");
     const NormQ8Params p{(int8_t*)q, scale, x, add, total, gain, ldq, ldx, ldadd, ldt, rows, width, eps};

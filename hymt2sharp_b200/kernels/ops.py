@@ -2367,6 +2367,7 @@ def dense_block(x, pre, residual, w_qkv, w_o, w_gate_up, w_down, q_gain, k_gain,
 
 
 # -- 8-bit integers with a scale a row --------------------------------------------------------------------------------------------
+Q8_MOST = 1 << 28         # rows, and entries of a row, that the 8-bit kernels take: they count bytes of a row in 32 bits
 Q8_MAX_INNER = 131071     # entries of a row that a product takes: 128 * 128 of them stay below 2^31
 
 
@@ -2383,6 +2384,8 @@ def _q8(t: torch.Tensor, scale: torch.Tensor, name: str) -> tuple:
     if t.dtype is not torch.int8 or len(shape) != 2:
         raise KernelError(f"{name} must be an int8 matrix, got {t.dtype} {tuple(shape)}")
     rows, width = shape
+    if rows > Q8_MOST or width > Q8_MOST:
+        raise KernelError(f"{name}: at most {Q8_MOST} rows of at most {Q8_MOST} entries, got {tuple(shape)}")
     ld, step = t.stride()
     if rows < 2:
         ld = (width + 15) & ~15

@@ -106,3 +106,12 @@ def test_plans_stay_within_the_machine(gated):
                     else:
                         assert T > 64 and p["splits"] == 1 and 64 <= p["width"] <= 256 and p["width"] % (64 if gated else 32) == 0 and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= sms
                         assert p["stages"] * (16384 + p["width"] * 64) + 32768 + 1024 == p["shared_bytes"] <= 226 * 1024
+
+
+@pytest.mark.parametrize("rows,width", [(1, ops.Q8_MOST + 1), (ops.Q8_MOST + 1, 1)])
+def test_matrices_beyond_what_is_counted(rows, width):
+    q = torch.empty_strided((rows, width), ((width + 15) & ~15, 1), dtype=torch.int8, device="meta")
+    s, x = torch.empty(rows, device="meta"), torch.empty(rows, width, device="meta")
+    for call in (lambda: ops.quantize_q8(q, s, x), lambda: ops.dequantize_q8(x, q, s), lambda: ops.rmsnorm_q8(q, s, x, torch.empty(width, device="meta"), 1e-5)):
+        with pytest.raises(ops.KernelError, match="at most"):
+            call()
