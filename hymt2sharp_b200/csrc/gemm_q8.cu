@@ -178,15 +178,21 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_base = tmem_base_s;
-    pdl_launch_dependents();            // (behind the allocation: a CTA of the next kernel cannot have taken this one's tensor memory)
+    // Tensor memory is taken once the kernel in front is through (a CTA of that one may have yet to take its own), and the next kernel released behind that.
+    uint32_t tmem_base = 0;
+    if (warp >= 1) {
+        pdl_wait();
+        if (warp == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+            pdl_launch_dependents();
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        asm volatile("bar.sync 2, %0;" ::"n"(32 + 32 * few_warps(BN)) : "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_base = tmem_base_s;
+    }
 
     if (warp == 0 && elect_one()) {
         auto load_weights = [&](int i) {
@@ -243,7 +249,6 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     } else if (warp >= 2) {
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        pdl_wait();             // C may still be in use by the kernel in front, and the scales come from it
         TC* C = (TC*)p.C;
         const int cols = min(BN, p.T - t0);
         // a lane of the fold has four neighbouring weight rows
@@ -421,7 +426,9 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     cluster_sync_all();                 // both CTAs' barriers and tensor memory are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_base_s;
-    pdl_launch_dependents();            // (behind the allocation: a CTA of the next kernel cannot have taken this one's tensor memory)
+    // (behind the allocation: a CTA of the next kernel cannot have taken this one's tensor memory; and beside this kernel's shared memory no CTA of the one in
+    // front fits that has yet to take its own)
+    pdl_launch_dependents();
 
     if (warp == 0 && elect_one()) {
         uint32_t s = 0, round = 0;

@@ -546,3 +546,36 @@ def test_weights_made_by_the_kernel_in_front():
             want = (a.double() @ q.double().T) * sa.double()[:, None] * s
             assert ((out.double() - want).abs() <= 6 * U * want.abs()).all()
     assert status.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("tokens", [1, 61, 128, 700])
+def test_products_of_both_kinds_follow_each_other(tokens):
+    """bfloat16 and 8-bit products directly behind one another, eager and replayed: each has tensor memory of its own, and none waits for another's."""
+    ops = _ops()
+    K, N = 512, 1024
+    status = ops.device_status(DEV)
+    x, w = _x(tokens, K, BF, 3), (0.1 * torch.randn(N, K, device=DEV)).to(BF)
+    (a, _), (b, _) = _fresh(tokens, K), _fresh(N, K)
+    sa, sb = torch.empty(tokens, device=DEV), torch.empty(N, device=DEV)
+    ops.quantize_q8(a, sa, x)
+    ops.quantize_q8(b, sb, w)
+    plain, short = torch.empty(tokens, N, dtype=BF, device=DEV), torch.empty(tokens, N, dtype=BF, device=DEV)
+
+    def both():
+        for _ in range(8):
+            ops.gemm_tc(plain, x, w, ops.EPILOGUE_STORE, status)
+            ops.gemm_q8_tc(short, a, sa, b, sb, ops.EPILOGUE_STORE, status, weights_settled=True)
+    both()
+    first = plain.clone(), short.clone()
+    want = (a.double() @ b.double().T) * sa.double()[:, None] * sb.double()
+    # two products with a scale, a conversion of a sum below 2^31: 4 half steps of float32, then one rounding to bfloat16
+    assert ((first[1].double() - want).abs() <= (4 * U + _half_step(BF)) * 1.01 * want.abs()).all()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for _ in range(5):
+        plain.zero_(), short.zero_()
+        graph.replay()
+        assert torch.equal(plain, first[0]) and torch.equal(short, first[1])
+    assert int(status[0]) == 0
