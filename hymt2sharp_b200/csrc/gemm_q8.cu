@@ -297,10 +297,21 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             for (int c0 = c_begin + warp - 2; c0 < c_end; c0 += WARPS * U) {
                 int4 part[U][R][NUM_ACC];
                 float sa[U];
+                [[maybe_unused]] float old[EPI == EPI_ACCUMULATE ? U : 1][4];       // what is added to: asked for with the sums, not behind them
 #pragma unroll
                 for (int k = 0; k < U; k++) {
                     const int c = c0 + k * WARPS;
                     sa[k] = c < c_end ? p.a_scale[t0 + c] : 0.f;
+                    if constexpr (EPI == EPI_ACCUMULATE) {
+                        const float* at = (const float*)C + (size_t)(t0 + c) * p.ldc + n4;
+                        if (vec && c < c_end) {
+                            const float4 v = *reinterpret_cast<const float4*>(at);
+                            old[k][0] = v.x; old[k][1] = v.y; old[k][2] = v.z; old[k][3] = v.w;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) old[k][i] = c < c_end && n4 + i < p.N ? at[i] : 0.f;
+                        }
+                    }
 #pragma unroll
                     for (int r = 0; r < R; r++)
 #pragma unroll
@@ -333,12 +344,11 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
                         for (int i = 0; i < 4; i++) if (n4 + i < p.N) y[0][i] = gated_at(p.glu, y[0][i], y[1][i], n4 + i, p.N);
                     }
+                    if constexpr (EPI == EPI_ACCUMULATE) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) y[0][i] = __fadd_rn(old[k][i], y[0][i]);
+                    }
                     if (vec) {
-                        if constexpr (EPI == EPI_ACCUMULATE) {
-                            const float4 old = *reinterpret_cast<const float4*>(dst);
-                            y[0][0] = __fadd_rn(old.x, y[0][0]); y[0][1] = __fadd_rn(old.y, y[0][1]);
-                            y[0][2] = __fadd_rn(old.z, y[0][2]); y[0][3] = __fadd_rn(old.w, y[0][3]);
-                        }
                         if constexpr (sizeof(TC) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0][0], y[0][1], y[0][2], y[0][3]);
                         else {
                             __nv_bfloat162 h[2] = {__floats2bfloat162_rn(y[0][0], y[0][1]), __floats2bfloat162_rn(y[0][2], y[0][3])};
@@ -347,7 +357,7 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            if (n4 + i < p.N) dst[i] = from_float<TC>(EPI == EPI_ACCUMULATE ? __fadd_rn(to_float(dst[i]), y[0][i]) : y[0][i]);
+                            if (n4 + i < p.N) dst[i] = from_float<TC>(y[0][i]);
                     }
                 }
             }
@@ -597,7 +607,10 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                             if constexpr (sizeof(TC) == 4) {
                                 float v;
                                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
-                                *dst = EPI == EPI_ACCUMULATE ? __fadd_rn(*dst, v) : v;
+                                // (added in memory, once a place: a read of the old value would be waited for row by row.  5,734 x 13,459 x 6,344 took
+                                // 1.1 ms so, and takes 0.44)
+                                if constexpr (EPI == EPI_ACCUMULATE) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(dst), "f"(v) : "memory");
+                                else *dst = v;
                             } else {
                                 unsigned short v;
                                 asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
