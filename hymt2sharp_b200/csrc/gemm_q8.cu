@@ -596,26 +596,34 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     used++;
                 } else {
-                    // rows that TMA does not write: a row's columns side by side, so that an access meets a few sectors and not 32
+                    // rows that TMA does not write: a row's columns side by side, so that an access meets a few sectors and not 32 (4,076 x 4,353 x 768 25 us,
+                    // with the reads out of shared memory one behind the other 34, and 4,352 columns by TMA 19)
                     __syncwarp();
-                    const int col = lane % PIECE, at = col * (int)sizeof(TC);
-#pragma unroll 4
-                    for (int row = lane / PIECE; row < 32; row += 32 / PIECE) {
-                        const uint32_t from = out + row * PIECE_BYTES + ((((at >> 4) ^ ((row >> 1) & 3)) << 4) | (at & 15));
-                        if (t_first + row < p.T && n + col < p.N) {
-                            TC* dst = C + (size_t)(t_first + row) * p.ldc + n + col;
-                            if constexpr (sizeof(TC) == 4) {
-                                float v;
-                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
-                                // (added in memory, once a place: a read of the old value would be waited for row by row.  5,734 x 13,459 x 6,344 took
-                                // 1.1 ms so, and takes 0.44)
-                                if constexpr (EPI == EPI_ACCUMULATE) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(dst), "f"(v) : "memory");
-                                else *dst = v;
-                            } else {
-                                unsigned short v;
-                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-                                *dst = __ushort_as_bfloat16(v);
+                    constexpr int ROWS = 32 / PIECE, BATCH = 8;            // rows an access, accesses whose reads are under way together
+                    const int col = lane % PIECE, first = lane / PIECE, at = col * (int)sizeof(TC);
+                    const int rows = n + col < p.N ? p.T - t_first - first : 0;
+                    TC* dst = C + (size_t)(t_first + first) * p.ldc + n + col;
+#pragma unroll
+                    for (int i0 = 0; i0 < 32 / ROWS; i0 += BATCH) {
+                        TC v[BATCH];
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) {
+                            const int row = (i0 + i) * ROWS;                // (row + first has the same place in the swizzle)
+                            const uint32_t from = out + (row + first) * PIECE_BYTES + ((((at >> 4) ^ ((row >> 1) & 3)) << 4) | (at & 15));
+                            if constexpr (sizeof(TC) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(from) : "memory");
+                            else {
+                                unsigned short h;
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from) : "memory");
+                                v[i] = __ushort_as_bfloat16(h);
                             }
+                        }
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++, dst += ROWS * p.ldc) {
+                            if ((i0 + i) * ROWS >= rows) continue;
+                            // (added in memory, once a place: a read of the old value would be waited for row by row.  5,734 x 13,459 x 6,344 took
+                            // 1.1 ms so, and takes 0.44)
+                            if constexpr (EPI == EPI_ACCUMULATE) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(dst), "f"(v[i]) : "memory");
+                            else *dst = v[i];
                         }
                     }
                 }
