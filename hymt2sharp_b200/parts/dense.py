@@ -88,7 +88,7 @@ def takes_rows8(block) -> bool:
 
 def _rows8(linear, rows: int, cols: int) -> bool:
     # (as parts.linear8.make_linear lays them out; a row's distance is a multiple of 16 also where there is one row)
-    return type(linear) is Linear8 and linear.weight.shape == (rows, cols) and linear.weight.stride() == ((cols + 15) & ~15, 1)
+    return type(linear) is Linear8 and linear.settled and linear.weight.shape == (rows, cols) and linear.weight.stride() == ((cols + 15) & ~15, 1)
 
 
 def try_block_rows8(block, residual: torch.Tensor, ctx, slot) -> bool:

@@ -48,11 +48,12 @@ class Rows8:
 
 class Linear8:
     """y = epilogue(x @ W^T) with W in 8-bit integers [out, in] and a scale a row; epilogue, role, glu and glu_bias as for Linear.  `dtype` is what
-    its outputs have where the call does not say (its inputs may be 8-bit rows, which have none)."""
+    its outputs have where the call does not say (its inputs may be 8-bit rows, which have none).  `settled`: whoever made the weights has waited for them and
+    leaves them as they are, so that a product may fetch them while the kernel in front of it runs; without it they may come from that very kernel."""
 
     def __init__(self, weight: Rows8, dtype: torch.dtype, epilogue: int = ops.EPILOGUE_STORE, role: str | None = None, glu: "ops.GluRule | None" = None,
-                 glu_bias: torch.Tensor | None = None):
-        self.rows, self.dtype = weight, dtype
+                 glu_bias: torch.Tensor | None = None, settled: bool = False):
+        self.rows, self.dtype, self.settled = weight, dtype, settled
         self.weight, self.scale = weight.q, weight.scale
         self.epilogue, self.role, self.glu, self.glu_bias = epilogue, role, glu, glu_bias
         self.out_features = weight.shape[0] // 2 if epilogue == ops.EPILOGUE_SWIGLU else weight.shape[0]
@@ -66,7 +67,7 @@ class Linear8:
             if out is None:
                 out = torch.empty((x.shape[0], self.out_features), dtype=out_dtype or self.dtype, device=x.device)
             ops.gemm_q8_tc(out, rows.q, rows.scale, self.weight, self.scale, self.epilogue, ops.device_status(out.device), self.glu, self.glu_bias,
-                           weights_settled=True)
+                           weights_settled=self.settled)
         finally:
             ops.tag = None
         return out
@@ -85,13 +86,13 @@ def make_linear(weights: str | None, weight: torch.Tensor, device, dtype: torch.
         return Linear(compute_form(weight, device, dtype), epilogue, **more)
     rows = Rows8.of(weight.to(device).contiguous())
     torch.cuda.current_stream(rows.device).synchronize()      # (every later product may fetch them before the kernel in front of it is through)
-    return Linear8(rows, dtype, epilogue, **more)
+    return Linear8(rows, dtype, epilogue, settled=True, **more)
 
 
 def same_weight(linear, epilogue: int):
     """Another product with the matrix of `linear`."""
     if isinstance(linear, Linear8):
-        return Linear8(linear.rows, linear.dtype, epilogue, role=linear.role)
+        return Linear8(linear.rows, linear.dtype, epilogue, role=linear.role, settled=linear.settled)
     return Linear(linear.weight, epilogue, role=linear.role)
 
 
