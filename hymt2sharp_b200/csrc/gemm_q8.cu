@@ -502,15 +502,16 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         TC* C = (TC*)p.C;
         const bool plain = p.glu.kind == GLU_SILU && !p.glu.bias;
         int j = 0, used = 0;
-        // the token's scale, and the scale of one column of a piece a lane (gated: of its gate and its up row): fetched a tile and a piece ahead
+        // the token's scale, and the scale of one column of a piece a lane (gated: of its gate and its up row): fetched a tile and a piece ahead.  (Plain
+        // loads: the kernel in front may have been writing them when this one was started, so they are not read-only data, and stay behind the wait.)
         auto first_token = [&](int tile) { return (tile % tiles_t) * 2 * TILE_M + rank * TILE_M + quarter * 32; };
         auto token_scale = [&](int tile) {
             const int t = first_token(tile) + lane;
-            return tile < num_tiles && t < p.T ? __ldg(p.a_scale + t) : 0.f;
+            return tile < num_tiles && t < p.T ? p.a_scale[t] : 0.f;
         };
         auto column_scale = [&](int tile, int c, int h) {
             const int n = (tile / tiles_t) * OUT_COLS + c + lane;
-            return tile < num_tiles && c < OUT_COLS && lane < PIECE && n < p.N ? __ldg(p.w_scale + (size_t)h * p.N + n) : 0.f;
+            return tile < num_tiles && c < OUT_COLS && lane < PIECE && n < p.N ? p.w_scale[(size_t)h * p.N + n] : 0.f;
         };
         float sa_next = token_scale(pair), ws_next = column_scale(pair, side * PIECE, 0), us_next = GATED ? column_scale(pair, side * PIECE, 1) : 0.f;
         for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
