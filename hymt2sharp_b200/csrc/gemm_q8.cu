@@ -32,7 +32,13 @@ struct GemmQ8Params {
     int tma_out;             // many tokens: C leaves by TMA
     int* status;
     GluRule glu;
+    uint32_t wait_limit;     // FAULT: tries of a wait before it gives up,
+    int withhold_block;      // and a k block whose copies are announced and never made
 };
+// FAULT: kernels for hymt2_gemm_q8_debug, whose waits have a limit of the launch's (read from the arguments it costs every wait of every launch: 2,048 x 2,048
+// for a token 4.2 us against 4.0) and which copy every block but one.
+template <bool FAULT> __device__ __forceinline__ uint32_t wait_limit(const GemmQ8Params& p) { return FAULT ? p.wait_limit : WAIT_LIMIT; }
+template <bool FAULT> __device__ __forceinline__ uint32_t landing_limit(const GemmQ8Params& p) { return FAULT ? p.wait_limit : 1u << 16; }
 
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
@@ -145,7 +151,7 @@ __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t local_addr, uint32_t r
 __host__ __device__ constexpr int few_warps(int bn) { return bn >= 64 ? 8 : 4; }      // that drain the sums (behind warp 0, TMA, and warp 1, MMAs)
 constexpr int MAX_RANKS = 8;           // a portable cluster
 
-template <int BN, int EPI, typename TC>
+template <int BN, int EPI, typename TC, bool FAULT = false>
 __global__ void __launch_bounds__(64 + 32 * few_warps(BN))
 gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, GemmQ8Params p) {
     constexpr int NUM_ACC = EPI == EPI_GATED ? 2 : 1;
@@ -194,14 +200,17 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         tmem_base = tmem_base_s;
     }
 
+    int issued = 0;                     // k blocks that were announced (in the thread that copies)
     if (warp == 0 && elect_one()) {
         auto load_weights = [&](int i) {
             const uint32_t bar = full0 + 8 * (i % stages), dst = tiles + (i % stages) * STAGE_BYTES;
             const int k = (kb_begin + i) * BLOCK_K;
+            if (FAULT && kb_begin + i == p.withhold_block) return;
             tma_load_2d(dst, &map_w, bar, k, n0);
             if (NUM_ACC == 2) tma_load_2d(dst + A_TILE_BYTES, &map_w, bar, k, p.N + n0);
         };
         auto load_tokens = [&](int i) {
+            if (FAULT && kb_begin + i == p.withhold_block) return;
             tma_load_2d(tiles + (i % stages) * STAGE_BYTES + NUM_ACC * A_TILE_BYTES, &map_a, full0 + 8 * (i % stages), (kb_begin + i) * BLOCK_K, t0);
         };
         // the first ring of weights before the wait for the kernel in front, where they do not come from it
@@ -213,25 +222,25 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         if (p.early) pdl_wait();
         for (int i = 0; i < ahead; i++) load_tokens(i);
-        int issued = ahead;
+        issued = ahead;
         for (int i = ahead; i < my_blocks; i++) {
             const int s = i % stages;
-            if (!mbar_wait(empty0 + 8 * s, ((i / stages) & 1) ^ 1, abort_flag, p.status, 151)) break;
+            if (!mbar_wait(empty0 + 8 * s, ((i / stages) & 1) ^ 1, abort_flag, p.status, 151, wait_limit<FAULT>(p))) break;
             mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
             load_weights(i);
             load_tokens(i);
             issued = i + 1;
         }
-        if (*abort_flag)        // copies that are in flight must land before the CTA's shared memory goes away
-            for (int i = max(0, issued - stages); i < issued; i++)
-                for (uint32_t t = 0; t < (1u << 16) && !mbar_try_wait(full0 + 8 * (i % stages), (i / stages) & 1); t++) {}
     } else if (warp == 1 && elect_one()) {
         constexpr uint64_t K_STEP = UMMA_K >> 4, A2_STEP = A_TILE_BYTES >> 4, B_STEP = (NUM_ACC * A_TILE_BYTES) >> 4;
         const uint64_t desc0 = desc_k_major(tiles);
         uint32_t s = 0, phase = 0;
         bool seen = false;
         for (int i = 0; i < my_blocks; i++) {
-            if (!seen && !mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152)) break;
+            if (!seen && !mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152, wait_limit<FAULT>(p))) {
+                __threadfence_block();          // whoever meets the barrier below also meets the abort flag
+                break;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t adesc = desc0 + (uint64_t)s * (uint64_t)(STAGE_BYTES >> 4), bdesc = adesc + B_STEP;
             const uint32_t s_next = s + 1 == (uint32_t)stages ? 0 : s + 1, phase_next = s_next ? phase : phase ^ 1;
@@ -260,8 +269,10 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             for (int i = 0; i < 4; i++) sw[h][i] = n4 + i < p.N ? p.w_scale[(size_t)h * p.N + n4 + i] : 0.f;
         const bool vec = n4 + 4 <= p.N && (p.ldc & 3) == 0 && ((uintptr_t)C & (4 * sizeof(TC) - 1)) == 0;
 
-        const bool ok = my_blocks > 0 ? mbar_wait(done_bar, 0, abort_flag, p.status, 153) : true;
-        __syncwarp();
+        // (done_bar completes for an issuer that gave up too, once the MMAs that it did issue are through.  One answer for the warp: a load of tensor memory
+        // takes all of it)
+        const bool done = my_blocks > 0 ? mbar_wait(done_bar, 0, abort_flag, p.status, 153, wait_limit<FAULT>(p)) : true;
+        const bool ok = __all_sync(0xffffffffu, done && !*abort_flag);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // the sums -> this CTA's shared memory (the ring is free now), [column][row]
         constexpr int CH = BN >= 32 ? 32 : 16, GROUPS = few_warps(BN) / 4;
@@ -285,6 +296,12 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         __syncwarp();
         if (p.splits > 1) cluster_sync_all();
         else asm volatile("bar.sync 1, %0;" ::"n"(32 * few_warps(BN)) : "memory");
+        // Where one of the cluster's CTAs gave up, the tile becomes NaN: every wait lies in front of this barrier, so the ranks' abort flags say it.  They are asked
+        // for in front of the sums and looked at behind them, by a factor and not a branch (64 tokens, 2,048 x 2,048: 4.8 us, with a branch 4.9, without either 4.7).
+        int gave_up = 0;
+        if (p.splits == 1) gave_up = *abort_flag;
+        else if (lane < p.splits)
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(gave_up) : "r"(at_rank(smem_u32(&abort_s), lane)) : "memory");
         // every CTA of the cluster takes a share of the tokens, adds all ranks' sums for them and writes them out; a warp has a token, a lane four
         // weight rows.  The way to another CTA's memory is long (one token at a time took 170 ns a token), so the sums of U tokens and R ranks are
         // asked for together: many tokens a warp where there are few ranks, and the other way round.
@@ -326,11 +343,13 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                             }
                         }
                 }
+                const bool none = __any_sync(0xffffffffu, gave_up);
 #pragma unroll
                 for (int k = 0; k < U; k++) {
                     const int c = c0 + k * WARPS;
                     if (c >= c_end) break;
                     float y[NUM_ACC][4];
+                    if (none) sa[k] = __uint_as_float(0x7fc00000u);
 #pragma unroll
                     for (int h = 0; h < NUM_ACC; h++) {
                         int4 sum = part[k][0][h];
@@ -368,13 +387,25 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         else fold(std::integral_constant<int, 1>{}, std::integral_constant<int, MAX_RANKS>{});
         __syncwarp();
     }
+    // Where a role gave up, copies may be in flight: they must land before the CTA's shared memory goes away.  (Looked at once every wait of the CTA is behind
+    // it, while the sums are folded; a wait for the copies in every launch took 2,048 x 2,048 for a token from 4.0 to 4.4 us.)
+    auto landed = [&] {
+        if (warp == 0 && *abort_flag)
+            for (int i = max(0, issued - stages); i < issued; i++)
+                for (uint32_t t = 0; t < landing_limit<FAULT>(p) && !mbar_try_wait(full0 + 8 * (i % stages), (i / stages) & 1); t++) {}
+        __syncwarp();
+    };
     if (p.splits > 1) {         // no CTA leaves before its peers have read its sums; the other warps come to both barriers too
         __syncwarp();
-        if (warp < 2) cluster_sync_all();
+        if (warp < 2) {
+            cluster_sync_all();
+            landed();
+        }
         cluster_sync_all();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (p.splits == 1) landed();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
@@ -390,7 +421,7 @@ constexpr int PAIR_BN = 256;           // the widest tile: the accumulators lie 
 constexpr int PIECE_BYTES = 64;        // a token's piece of output columns: 32 of bfloat16, 16 of float32
 constexpr int OUT_BUFFER = 32 * PIECE_BYTES, OUT_BYTES = 8 * 2 * OUT_BUFFER;   // a warp has two buffers that TMA writes out
 
-template <int EPI, typename TC>
+template <int EPI, typename TC, bool FAULT = false>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
                     GemmQ8Params p) {
@@ -450,24 +481,25 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             // the even CTA brings the first half of the weight rows, the odd one the second; of gated rows the gates and the ups
             const int w_row = (tile / tiles_t) * OUT_COLS + rank * (GATED ? p.N : bn / 2);
             for (int kb = 0; kb < num_k_blocks; kb++) {
-                if (round > 0 && !seen && !mbar_wait(empty0 + 8 * s, (round & 1) ^ 1, abort_flag, p.status, 151)) break;
+                if (round > 0 && !seen && !mbar_wait(empty0 + 8 * s, (round & 1) ^ 1, abort_flag, p.status, 151, wait_limit<FAULT>(p))) break;
                 const uint32_t bar = even_full0 + 8 * s, a_dst = tiles + s * STAGE_BYTES;
                 const uint32_t s_next = s + 1 == (uint32_t)stages ? 0 : s + 1, round_next = s_next ? round : round + 1;
                 seen = round_next > 0 && mbar_look(empty0 + 8 * s_next, (round_next & 1) ^ 1);
                 if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
-                tma_load_2d_pair(a_dst + A_TILE_BYTES, &map_w, bar, kb * BLOCK_K, w_row);
+                if (!FAULT || kb != p.withhold_block) tma_load_2d_pair(a_dst + A_TILE_BYTES, &map_w, bar, kb * BLOCK_K, w_row);
                 if (first && p.early) pdl_wait();
                 first = false;
-                tma_load_2d_pair(a_dst, &map_a, bar, kb * BLOCK_K, a_row);
+                if (!FAULT || kb != p.withhold_block) tma_load_2d_pair(a_dst, &map_a, bar, kb * BLOCK_K, a_row);
                 s = s_next;
                 round = round_next;
             }
         }
-        if (rank == 0 && *abort_flag)   // copies in flight (both CTAs' are counted here) must land before the shared memory goes away
+        // copies (both CTAs' are counted here) must land before the shared memory goes away, whatever became of the roles that wait for them
+        if (rank == 0)
             for (int back = 0; back < stages && (round > 0 || s > 0); back++) {
                 if (s == 0) { s = stages; round--; }
                 s--;
-                for (uint32_t t = 0; t < (1u << 16) && !mbar_try_wait(full0 + 8 * s, round & 1); t++) {}
+                for (uint32_t t = 0; t < landing_limit<FAULT>(p) && !mbar_try_wait(full0 + 8 * s, round & 1); t++) {}
             }
     } else if (warp == 1 && rank == 0 && elect_one()) {
         const uint64_t desc0 = desc_k_major(tiles);
@@ -476,11 +508,11 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         int j = 0;
         for (int tile = pair; tile < num_tiles; tile += pairs, j++) {
             const int buf = j & 1;
-            if (j >= 2 && !mbar_wait(acc_empty0 + 8 * buf, (uint32_t)(((j >> 1) - 1) & 1), abort_flag, p.status, 154)) break;
+            if (j >= 2 && !mbar_wait(acc_empty0 + 8 * buf, (uint32_t)(((j >> 1) - 1) & 1), abort_flag, p.status, 154, wait_limit<FAULT>(p))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             bool ok = true;
             for (int kb = 0; kb < num_k_blocks; kb++) {
-                if (!seen && !(ok = mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152))) break;
+                if (!seen && !(ok = mbar_wait(full0 + 8 * s, phase, abort_flag, p.status, 152, wait_limit<FAULT>(p)))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t adesc = desc0 + (uint64_t)s * (uint64_t)(STAGE_BYTES >> 4), bdesc = adesc + (A_TILE_BYTES >> 4);
                 const uint32_t s_next = s + 1 == (uint32_t)stages ? 0 : s + 1, phase_next = s_next ? phase : phase ^ 1;
@@ -523,7 +555,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             sa_next = token_scale(tile + pairs);
             ws_next = column_scale(tile + pairs, side * PIECE, 0);
             if constexpr (GATED) us_next = column_scale(tile + pairs, side * PIECE, 1);
-            const bool landed = mbar_wait(acc_full0 + 8 * buf, (uint32_t)((j >> 1) & 1), abort_flag, p.status, 153);
+            const bool landed = mbar_wait(acc_full0 + 8 * buf, (uint32_t)((j >> 1) & 1), abort_flag, p.status, 153, wait_limit<FAULT>(p));
             if (!__all_sync(0xffffffffu, landed)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * PAIR_BN;
@@ -796,7 +828,7 @@ int launch_cluster(dim3 grid, int threads, dim3 cluster, size_t smem, cudaStream
     return hymt2_check_launch("gemm_q8_tc");
 }
 
-template <int EPI, typename TC>
+template <int EPI, typename TC, bool FAULT = false>
 int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const Plan& pl, cudaStream_t stream) {
     CUtensorMap ma, mw, mc{};
     const long w_rows = EPI == EPI_GATED ? 2L * p.N : p.N;
@@ -805,7 +837,10 @@ int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const 
     if (pl.few) {
         const dim3 grid(pl.tiles_n, pl.tiles_t, pl.splits), cluster(1, 1, pl.splits);
         const int threads = 64 + 32 * few_warps(pl.bn);
-        switch (pl.bn) {
+        if constexpr (FAULT) {
+            HYMT2_REQUIRE(pl.bn == 16, "gemm_q8_debug: at most 16 tokens, or many");
+            return launch_cluster<gemm_q8_few_kernel<16, EPI, TC, true>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
+        } else switch (pl.bn) {
             case 16: return launch_cluster<gemm_q8_few_kernel<16, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
             case 32: return launch_cluster<gemm_q8_few_kernel<32, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
             case 64: return launch_cluster<gemm_q8_few_kernel<64, EPI, TC>>(grid, threads, cluster, pl.smem, stream, mw, ma, p);
@@ -815,7 +850,7 @@ int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const 
     // (TMA writes whole pieces of 16 bytes: where the last of a row is not whole, it would write what lies between the rows)
     p.tma_out = (uintptr_t)p.C % 16 == 0 && p.ldc * (long)sizeof(TC) % 16 == 0 && p.N * (long)sizeof(TC) % 16 == 0;
     if (p.tma_out) HYMT2_REQUIRE(make_map_out(&mc, p.C, sizeof(TC) == 2, p.T, p.N, p.ldc), "gemm_q8_tc: cuTensorMapEncodeTiled refused the output");
-    return launch_cluster<gemm_q8_pair_kernel<EPI, TC>>(dim3(pl.ctas), PAIR_THREADS, dim3(2, 1, 1), pl.smem, stream, ma, mw, mc, p);
+    return launch_cluster<gemm_q8_pair_kernel<EPI, TC, FAULT>>(dim3(pl.ctas), PAIR_THREADS, dim3(2, 1, 1), pl.smem, stream, ma, mw, mc, p);
 }
 
 }  // namespace
@@ -845,9 +880,28 @@ HYMT2_API int hymt2_gemm_q8_tc(void* C, int c_dtype, const void* A, const float*
     const Plan pl = make_plan(T, N, K, epilogue == EPI_GATED, sm_count_of_current_device());
     HYMT2_REQUIRE(pl.tiles_t <= 65535, "gemm_q8_tc: grid too large");
     const GemmQ8Params p{C, a_scale, w_scale, ldc, T, N, K, pl.bn, pl.stages, pl.splits, pl.k_blocks_per_split, weights_settled, 0, status,
-                         GluRule{glu_kind, glu_limit, glu_alpha, glu_bias}};
+                         GluRule{glu_kind, glu_limit, glu_alpha, glu_bias}, WAIT_LIMIT, -1};
     if (epilogue == EPI_ACCUMULATE) return run<EPI_ACCUMULATE, float>(A, W, lda, ldw, p, pl, stream);
     if (epilogue == EPI_STORE)
         return c_dtype == HYMT2_F32 ? run<EPI_STORE, float>(A, W, lda, ldw, p, pl, stream) : run<EPI_STORE, __nv_bfloat16>(A, W, lda, ldw, p, pl, stream);
     return c_dtype == HYMT2_F32 ? run<EPI_GATED, float>(A, W, lda, ldw, p, pl, stream) : run<EPI_GATED, __nv_bfloat16>(A, W, lda, ldw, p, pl, stream);
+}
+
+// The same product with a fault put in on purpose, for a test of the waits: the copies of k block `withhold_block` are announced and never made, and every
+// wait gives up after `wait_limit` tries (a few thousand: milliseconds).  The waits for that block, for the stages behind it and for the sums then run out: a
+// CTA whose wait does writes 151, 152 or 153 into the status word and raises its abort flag, every role leaves its loop, every CTA comes to the cluster's
+// barriers, C's tile is NaN (few tokens) or left as it was, copies in flight land, tensor memory is freed and the kernel returns.  Only sums added into float32 and
+// gated products into bfloat16, of up to 16 tokens or of many, on at most 8 CTAs are taken.
+HYMT2_API int hymt2_gemm_q8_debug(void* C, int c_dtype, const void* A, const float* a_scale, const void* W, const float* w_scale, int T, int N, int K,
+                                  long lda, long ldw, long ldc, int epilogue, int* status, cudaStream_t stream, int wait_limit, int withhold_block) {
+    HYMT2_REQUIRE(T > 0 && N > 0 && K > 0 && K <= MAX_K && status != nullptr, "gemm_q8_debug: bad sizes T=%d N=%d K=%d", T, N, K);
+    HYMT2_REQUIRE(wait_limit > 0 && wait_limit <= (1 << 16), "gemm_q8_debug: wait_limit %d must be in [1, 65536]", wait_limit);
+    HYMT2_REQUIRE(withhold_block >= 0 && withhold_block < (K + BLOCK_K - 1) / BLOCK_K, "gemm_q8_debug: K has no block %d", withhold_block);
+    const Plan pl = make_plan(T, N, K, epilogue == EPI_GATED, sm_count_of_current_device());
+    HYMT2_REQUIRE(pl.ctas <= MAX_RANKS, "gemm_q8_debug: at most %d CTAs", MAX_RANKS);
+    const GemmQ8Params p{C, a_scale, w_scale, ldc, T, N, K, pl.bn, pl.stages, pl.splits, pl.k_blocks_per_split, 0, 0, status, GluRule{}, (uint32_t)wait_limit,
+                         withhold_block};
+    if (epilogue == EPI_ACCUMULATE && c_dtype == HYMT2_F32) return run<EPI_ACCUMULATE, float, true>(A, W, lda, ldw, p, pl, stream);
+    if (epilogue == EPI_GATED && c_dtype == HYMT2_BF16) return run<EPI_GATED, __nv_bfloat16, true>(A, W, lda, ldw, p, pl, stream);
+    HYMT2_REQUIRE(false, "gemm_q8_debug: epilogue %d with output type %d is not built", epilogue, c_dtype);
 }

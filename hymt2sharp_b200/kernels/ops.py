@@ -2501,6 +2501,23 @@ def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: tor
                                    epilogue, 1 if weights_settled else 0, status.data_ptr(), _raw_stream(), *rule), "gemm_q8_tc")
 
 
+def gemm_q8_debug(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int, status: torch.Tensor,
+                  wait_limit: int, withhold_block: int) -> None:
+    """gemm_q8_tc with a fault put in on purpose: the copies of k block `withhold_block` are announced and never made, and every wait gives up after
+    `wait_limit` tries.  The kernel must set status[0] to 151, 152 or 153, write no number into `out` (of few tokens NaN, of many nothing), free what it holds and
+    return.  Only sums added into float32 and gated products into bfloat16, of up to 16 tokens or of many, by at most eight CTAs are taken."""
+    T, K, lda = _q8(a, a_scale, "a")
+    rows_w, inner, ldw = _q8(w, w_scale, "w")
+    N = rows_w // 2 if epilogue == EPILOGUE_SWIGLU else rows_w
+    ldo = _plain_rows(out, "out", T, N)
+    if inner != K:
+        raise KernelError("gemm_q8_debug: operands are not taken")
+    _on_current_device("gemm_q8_debug", out, a, a_scale, w, w_scale, status)
+    _check(_lib().hymt2_gemm_q8_debug(_ptr(out), c_int(dtype_code(out.dtype)), _ptr(a), _ptr(a_scale), _ptr(w), _ptr(w_scale), c_int(T), c_int(N), c_int(K),
+                                      c_long(lda), c_long(ldw), c_long(ldo), c_int(epilogue), _ptr(status), _stream(), c_int(wait_limit),
+                                      c_int(withhold_block)), "gemm_q8_debug")
+
+
 def gemm_q8_describe(tokens: int, out_features: int, inner: int, gated: bool, sm_count: int = 0) -> dict:
     """How gemm_q8_tc would run a product (of 2 * out_features weight rows if gated) on a device of sm_count SMs (0: the current one)."""
     out = (c_long * 7)()
