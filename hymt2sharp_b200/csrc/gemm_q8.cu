@@ -857,9 +857,9 @@ int run(const void* A, const void* W, long lda, long ldw, GemmQ8Params p, const 
 
 // How a product of T tokens, N outputs (gated: of 2N weight rows) and K would be run on a device of sm_count SMs (0: the current one): out[0] the kernel for few
 // tokens, [1] the tile's other side (tokens, or a pair's weight rows), [2] stages of the ring, [3] the cut of K, [4] k blocks of a part, [5] CTAs, [6] bytes of
-// shared memory.  Nothing is launched.
+// shared memory.  Nothing is launched.  (A device has room for a pair of CTAs.)
 HYMT2_API int hymt2_gemm_q8_describe(int T, int N, int K, int gated, int sm_count, long* out) {
-    HYMT2_REQUIRE(T > 0 && N > 0 && K > 0 && K <= MAX_K && out, "gemm_q8_describe: bad arguments");
+    HYMT2_REQUIRE(T > 0 && N > 0 && K > 0 && K <= MAX_K && sm_count != 1 && out, "gemm_q8_describe: bad arguments");
     const Plan pl = make_plan(T, N, K, gated != 0, sm_count > 0 ? sm_count : sm_count_of_current_device());
     const long v[7] = {pl.few, pl.bn, pl.stages, pl.splits, pl.k_blocks_per_split, pl.ctas, (long)pl.smem};
     for (int i = 0; i < 7; i++) out[i] = v[i];
