@@ -769,6 +769,7 @@ void plan_pairs(Plan& pl, int T, int N, int K, bool gated, int sm_count, int bn)
     pl.cost = 2500.0 + 10.0 * bn + (stream > memory ? stream : memory);
 }
 
+constexpr long MOST_TILES = 1L << 30;      // (they are counted in an int, some beyond the last)
 constexpr int FEW_MOST_TOKENS = 512;       // from here on pairs were the faster ones at every size swept
 
 Plan make_plan(int T, int N, int K, bool gated, int sm_count) {
@@ -878,7 +879,7 @@ HYMT2_API int hymt2_gemm_q8_tc(void* C, int c_dtype, const void* A, const float*
                   "gemm_q8_tc: epilogue %d with output type %d is not built", epilogue, c_dtype);
     HYMT2_REQUIRE(status != nullptr, "gemm_q8_tc: a status word is needed");
     const Plan pl = make_plan(T, N, K, epilogue == EPI_GATED, sm_count_of_current_device());
-    HYMT2_REQUIRE(pl.tiles_t <= 65535, "gemm_q8_tc: grid too large");
+    HYMT2_REQUIRE((long)pl.tiles_t * pl.tiles_n <= MOST_TILES, "gemm_q8_tc: too many tiles");
     const GemmQ8Params p{C, a_scale, w_scale, ldc, T, N, K, pl.bn, pl.stages, pl.splits, pl.k_blocks_per_split, weights_settled, 0, status,
                          GluRule{glu_kind, glu_limit, glu_alpha, glu_bias}, WAIT_LIMIT, -1};
     if (epilogue == EPI_ACCUMULATE) return run<EPI_ACCUMULATE, float>(A, W, lda, ldw, p, pl, stream);
