@@ -50,20 +50,22 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// x sigmoid(alpha x) by the hardware's approximate exponential and reciprocal (together within 2^-22 of the result and 2^-24 of the exponent's size).  The drain of
-// a gated tile is bound by its instructions: 2,048 x 6,144 gated x 2,048 took 74 us with an exact division and exponential, 64 with these.
-__device__ __forceinline__ float swish(float x, float alpha) {
+// x sigmoid(alpha x).  The drain of a gated tile is bound by its instructions (2,048 x 6,144 gated x 2,048 into bfloat16 took 74 us with an exact division and
+// exponential, 64 with approximate ones), so the reciprocal is the hardware's approximate one (a step of float32).  The exponential is too where the result becomes
+// bfloat16: it is off by 2^-22 and by 2^-24 of its argument's size, where that rounding is 2^-9.  What stays float32 has expf, so that far negative gates are as
+// good as near ones (8 half steps in all; the form with a division, common.cuh's silu_mul, 6): that product takes 43.2 us for 42.5, with the division 51.
+template <typename TC> __device__ __forceinline__ float swish(float x, float alpha) {
     float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-alpha * x)));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + (sizeof(TC) == 4 ? expf(-alpha * x) : __expf(-alpha * x))));
     return x * r;
 }
 // glu_at of common.cuh, but a NaN stays one under the clamps: it says that the row held one before it became integers
-__device__ __forceinline__ float gated_at(const GluRule& r, float g, float u, int n, int N) {
+template <typename TC> __device__ __forceinline__ float gated_at(const GluRule& r, float g, float u, int n, int N) {
     if (r.bias) { g = __fadd_rn(g, r.bias[n]); u = __fadd_rn(u, r.bias[N + n]); }
-    if (r.kind == GLU_SILU) return swish(g, 1.0f) * u;
+    if (r.kind == GLU_SILU) return swish<TC>(g, 1.0f) * u;
     g = min_nan(g, r.limit);
     u = min_nan(max_nan(u, -r.limit), r.limit);
-    return swish(g, r.alpha) * (u + 1.0f);
+    return swish<TC>(g, r.alpha) * (u + 1.0f);
 }
 // (products of their own and no FMA with what follows: both kernels give the same bits)
 __device__ __forceinline__ float scaled(int sum, float a, float w) { return __fmul_rn(__fmul_rn((float)sum, a), w); }
@@ -361,7 +363,7 @@ gemm_q8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     TC* dst = C + (size_t)(t0 + c) * p.ldc + n4;
                     if constexpr (EPI == EPI_GATED) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) if (n4 + i < p.N) y[0][i] = gated_at(p.glu, y[0][i], y[1][i], n4 + i, p.N);
+                        for (int i = 0; i < 4; i++) if (n4 + i < p.N) y[0][i] = gated_at<TC>(p.glu, y[0][i], y[1][i], n4 + i, p.N);
                     }
                     if constexpr (EPI == EPI_ACCUMULATE) {
 #pragma unroll
@@ -591,10 +593,10 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     scale_all(u, out + 128);
                     if (plain) {
 #pragma unroll
-                        for (int q = 0; q < PIECE; q++) y[q] = swish(y[q], 1.0f) * u[q];
+                        for (int q = 0; q < PIECE; q++) y[q] = swish<TC>(y[q], 1.0f) * u[q];
                     } else {
 #pragma unroll
-                        for (int q = 0; q < PIECE; q++) y[q] = n + q < p.N ? gated_at(p.glu, y[q], u[q], n + q, p.N) : 0.f;
+                        for (int q = 0; q < PIECE; q++) y[q] = n + q < p.N ? gated_at<TC>(p.glu, y[q], u[q], n + q, p.N) : 0.f;
                     }
                 }
                 // the token's 64 bytes, its 16-byte pieces where the 64-byte swizzle has them
