@@ -50,8 +50,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// x sigmoid(alpha x).  The drain of a gated tile is bound by its instructions (2,048 x 6,144 gated x 2,048 into bfloat16 took 74 us with an exact division and
-// exponential, 64 with approximate ones), so the reciprocal is the hardware's approximate one (a step of float32).  The exponential is too where the result becomes
+// x sigmoid(alpha x).  The drain of a gated tile is bound by its instructions (2,048 x 6,144 gated x 2,048 into bfloat16 takes 54 us with an exact division and
+// exponential, 39 with approximate ones), so the reciprocal is the hardware's approximate one (a step of float32).  The exponential is too where the result becomes
 // bfloat16: it is off by 2^-22 and by 2^-24 of its argument's size, where that rounding is 2^-9.  What stays float32 has expf, so that far negative gates are as
 // good as near ones (8 half steps in all; the form with a division, common.cuh's silu_mul, 6): that product takes 43.2 us for 42.5, with the division 51.
 template <typename TC> __device__ __forceinline__ float swish(float x, float alpha) {
@@ -711,8 +711,9 @@ struct Plan {
     double cost;             // ns
 };
 
-// What decides between the kernels, widths and cuts: estimates of a call's time in ns, fitted to sweeps of 1 to 6,000 tokens over eleven weights of 1,000 x 500
-// to 28,672 x 4,096 with every width and cut.  The rule's choice was within 4 % of the best one at 147 of 187 products and within 15 % at all others but two.
+// What decides between the kernels, widths and cuts: estimates of a call's time in ns, fitted to sweeps of 4 to 6,000 tokens over eleven weights of 1,000 x 500
+// to 28,672 x 4,096 with every cut, and pairs of 64, 128, 192 and 256 weight rows.  Against every cut and every width that it may choose (20 numbers of tokens
+// from 1 to 6,000) its choice was within 4 % of the best one at 186 of 220 products, within 10 % at 211 and within 19 % at all.
 // A CTA of the few-token kernel takes 200 ns a k block as long as its SM takes in less than 145 bytes a ns; partial sums cost by the number of ranks, and more
 // where more tokens are folded.  A pair by itself takes 1.07 ns a k block and weight row, and no less than its tiles' way from L2 (165 ns); with all SMs at
 // work (power, L2) 115 ns and 0.76 ns a weight row.

@@ -45,7 +45,7 @@ template <int V> __device__ __forceinline__ void q8_of(const float (&x)[V], cons
         code[i] = __float_as_uint(w);
         far = fmaxf(far, fabsf(__fmaf_rn(x[i], c.inv, WHOLE - w)));
     }
-    if (far > NEAR_BORDER) {      // (one float32 in 30,000)
+    if (far > NEAR_BORDER) {      // (3e-5 on each side of a border: one float32 in 17,000, eight of them one time in 2,100)
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float r = __uint_as_float(code[i]) - WHOLE, e = __fmaf_rn(x[i], c.inv, -r);
@@ -272,8 +272,8 @@ template <bool WARP, bool SUM> __device__ __forceinline__ void over_row(float& m
     if (SUM) ss = warp_sum(mine.y);
 }
 
-// MOST: the threads of a block at most; 256: a warp a row.  (Blocks an SM: with 39 registers a thread one block of 896 was there at a time, and
-// 8,192 x 14,336 took 179 us for 106 with two.)
+// MOST: the threads of a block at most; 256: a warp a row.  (Blocks an SM that the registers are to leave room for, compiled for one and as here: 8,192 x 14,336
+// bfloat16, three blocks of 448 threads, 81 and 72 us; 256 x 8,192, 4.4 and 3.4.)
 constexpr int quantize_blocks(int ch, int most, bool shift, int size) {
     return most == 256 || (ch == 4 && most == 1024) ? 1 : ch == 4 ? (size == 2 && !shift ? 3 : 2) : shift ? 1 : 2;
 }
@@ -500,9 +500,10 @@ __global__ void __launch_bounds__(256) dequantize_q8_kernel(TY* y, long ldy, con
 inline bool whole(const void* p, long ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
 
 // How a row is shared: groups of 8 entries a thread, a warp or a block a row, threads of a block.  Four groups a thread where there are more rows than two
-// blocks an SM, so that what a thread does once a row costs less (8,192 x 14,336 bfloat16 67 us, with two groups 91); fewer where a row's own way counts
-// (64 x 4,096 1.6 us with one group, 2.2 with two).  A norm takes one group as far as 512 threads go, then two (float32 and bfloat16 added: 8,192 x 4,096
-// 56 us, with two 62; 8,192 x 6,144 84 us, with one 89; 4,000 x 7,169 65, with one 103; 8,192 x 8,192 115, with one 110).
+// blocks an SM, so that what a thread does once a row costs less (8,192 x 14,336 bfloat16 72 us, with two groups 82; 8,192 x 8,192 40, with two 45, with one
+// 60); fewer where a row's own way counts (64 x 4,096 1.6 us with one group or two, 1.7 with four; 16 x 14,336 2.2, with four 2.3).  A norm takes one group as
+// far as 512 threads go, then two (float32 and bfloat16 added: 8,192 x 4,096 56 us, with two 62; 8,192 x 6,144 84 us, with one 89; 4,000 x 7,169 65, with one
+// 103; 8,192 x 8,192 115, with one 110).
 struct Share { int ch, threads, blocks; bool warp; };
 constexpr int FEW_ROWS = 296;
 Share share_of(int rows, int width, bool norm) {
