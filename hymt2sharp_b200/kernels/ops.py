@@ -2510,7 +2510,7 @@ def gemm_q8_debug(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: 
     rows_w, inner, ldw = _q8(w, w_scale, "w")
     N = rows_w // 2 if epilogue == EPILOGUE_SWIGLU else rows_w
     ldo = _plain_rows(out, "out", T, N)
-    if inner != K:
+    if inner != K or status.dtype != torch.int32 or status.numel() == 0:
         raise KernelError("gemm_q8_debug: operands are not taken")
     _on_current_device("gemm_q8_debug", out, a, a_scale, w, w_scale, status)
     _check(_lib().hymt2_gemm_q8_debug(_ptr(out), c_int(dtype_code(out.dtype)), _ptr(a), _ptr(a_scale), _ptr(w), _ptr(w_scale), c_int(T), c_int(N), c_int(K),
