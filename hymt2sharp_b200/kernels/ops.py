@@ -2476,7 +2476,7 @@ def gemm_q8_tc(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: tor
     added).  Store (float32 or bfloat16), accumulate (float32) or SwiGLU (w and w_scale have 2N rows, gates first; `glu` and `glu_bias` as for gemm_tc, with
     outputs of both types).  A token whose scale is NaN gets NaN.  At most Q8_MAX_INNER entries a row; `out` shares no memory with the operands.
     `weights_settled`: w was complete before the kernel in front of this call was launched, as a model's weights are; it is then fetched while that one
-    still runs."""
+    still runs.  A launch whose wait runs out sets status[0] (151 to 154) and writes no number from sums that did not come: NaN, or nothing."""
     T, K, lda = _q8(a, a_scale, "a")
     rows_w, inner, ldw = _q8(w, w_scale, "w")
     gated = epilogue == EPILOGUE_SWIGLU
